@@ -97,13 +97,13 @@ def build(jobs=None, verbose=True):
     return out
 
 
-BIND_SRC = os.path.join(CSRC, "bind", "hc_step_bind.cpp")
+BIND_SRCS = [os.path.join(CSRC, "bind", f) for f in ("hc_step_bind.cpp", "hc_pages_bind.cpp")]
 BIND_NAME = "hc_step_bind"
 
 
 def build_bind(verbose=True):
-    """The Python extension module of the decode loop's per-step call
-    (csrc/bind/hc_step_bind.cpp: host C++ against torch's headers, linked to
+    """The Python extension module of the decode loop's per-step call and the
+    paged operators (csrc/bind: host C++ against torch's headers, linked to
     libhotcold_hip.so beside it), built into OUT_DIR next to the library.
     Build the library first."""
     import torch.utils.cpp_extension as ce
@@ -117,7 +117,7 @@ def build_bind(verbose=True):
     # the build directory (where load() imports it once) the same library;
     # '$$' is ninja's escape of '$' and '\' the shell's
     rel = os.path.relpath(OUT_DIR, bdir)
-    ce.load(name=BIND_NAME, sources=[BIND_SRC], build_directory=bdir, extra_cflags=["-O3", f"-I{INCLUDE}"],
+    ce.load(name=BIND_NAME, sources=BIND_SRCS, build_directory=bdir, extra_cflags=["-O3", f"-I{INCLUDE}"],
             extra_ldflags=[f"-L{OUT_DIR}", "-lhotcold_hip", f"-Wl,-rpath,\\$$ORIGIN:\\$$ORIGIN/{rel}"],
             verbose=False)
     out = os.path.join(OUT_DIR, BIND_NAME + ".so")

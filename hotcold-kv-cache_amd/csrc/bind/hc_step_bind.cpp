@@ -88,6 +88,29 @@ std::tuple<at::Tensor, int64_t> decode_append_step(int64_t args_addr, const at::
   return {out, (int64_t)rc};
 }
 
+// The paged operators (hc_pages_bind.cpp).
+using OptTensor = c10::optional<at::Tensor>;
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, int64_t> extend_pages(
+    const at::Tensor& lens, const at::Tensor& new_lens, const at::Tensor& tables, const at::Tensor& free_pages,
+    const at::Tensor& free_count, int64_t page_size, int64_t num_tokens, const OptTensor& lens_out,
+    const OptTensor& count_out, int64_t stream);
+std::tuple<at::Tensor, at::Tensor, int64_t> release_pages(const at::Tensor& lens, const at::Tensor& keep_lens,
+                                                          const at::Tensor& tables, const at::Tensor& free_pages,
+                                                          const at::Tensor& free_count, int64_t page_size,
+                                                          const OptTensor& lens_out, const OptTensor& count_out,
+                                                          int64_t stream);
+int64_t append_paged(const at::Tensor& slots, const at::Tensor& k_new, const at::Tensor& v_new,
+                     const at::Tensor& k_pages, const at::Tensor& v_pages, int64_t stream);
+std::tuple<at::Tensor, OptTensor, int64_t> prefix_attention(
+    const at::Tensor& q, const OptTensor& k_prefix, const OptTensor& v_prefix, const at::Tensor& k_pages,
+    const at::Tensor& v_pages, const at::Tensor& tables, const at::Tensor& lens, double scaling,
+    const OptTensor& cu_new, const c10::optional<int64_t>& max_new, const OptTensor& prefix_lens,
+    const OptTensor& out, bool with_lse, int64_t stream);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_append_step", &decode_append_step, "the per-step half of hc_decode_attn_append_packed");
+  m.def("extend_pages", &extend_pages, "hc_extend_pages on tensors");
+  m.def("release_pages", &release_pages, "hc_release_pages on tensors");
+  m.def("append_paged", &append_paged, "hc_append_paged on tensors");
+  m.def("prefix_attention", &prefix_attention, "hc_prefix_attn on tensors");
 }

@@ -197,6 +197,15 @@ SIGNATURES = {
     "hc_gather_evict_bytes": (_i64, [_i64, _i64, _i64, _i64]),
     "hc_gather_evict": (_int, [_int, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64,
                                _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
+    # pages behind a shared prompt
+    "hc_extend_pages": (_int, [_i64, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp,
+                               _vp]),
+    "hc_release_pages": (_int, [_i64, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "hc_append_paged": (_int, [_int, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64,
+                               _vp, _i64, _i64, _i64, _i64, _i64, _vp]),
+    "hc_prefix_attn_workspace_size": (_i64, [_vp]),
+    "hc_prefix_attn": (_int, [_vp, _vp]),
+    "hc_prefix_attn_args_size": (_i64, []),
     # host cold store
     "hc_cold_create": (_vp, [_i64, _i64, _i64, _i64, _i64, _int]),
     "hc_cold_destroy": (None, [_vp]),
@@ -250,6 +259,18 @@ class DecodeH2OEvictArgs(ctypes.Structure):
         ("workspace_bytes num_splits", _i64)) for n in names.split()]
 
 
+class PrefixAttnArgs(ctypes.Structure):
+    """ctypes mirror of hc_prefix_attn_args (include/hotcold_hip.h): every
+    field 8 bytes, in the header's order."""
+    _fields_ = [(n, t) for names, t in (
+        ("dtype N B Hq Hk D", _i64), ("q", _vp), ("q_sn q_sh", _i64), ("k_prefix", _vp), ("kp_sh kp_ss", _i64),
+        ("v_prefix", _vp), ("vp_sh vp_ss prefix_rows", _i64), ("prefix_lens k_pages", _vp),
+        ("kg_sp kg_sh kg_ss", _i64), ("v_pages", _vp), ("vg_sp vg_sh vg_ss num_pages page_size", _i64),
+        ("tables", _vp), ("t_sb table_width", _i64), ("lens cu_new", _vp), ("max_new", _i64), ("scaling", _dbl),
+        ("out", _vp), ("o_sn o_sh", _i64), ("lse", _vp), ("l_sn l_sh", _i64), ("workspace", _vp),
+        ("workspace_bytes", _i64)) for n in names.split()]
+
+
 def library_path():
     return _LIB_PATH
 
@@ -275,6 +296,8 @@ def lib():
             raise RuntimeError("hotcold_kv: hc_decode_append_args layout differs between the library and the binding")
         if handle.hc_decode_h2o_evict_args_size() != ctypes.sizeof(DecodeH2OEvictArgs):
             raise RuntimeError("hotcold_kv: hc_decode_h2o_evict_args layout differs between the library and the binding")
+        if handle.hc_prefix_attn_args_size() != ctypes.sizeof(PrefixAttnArgs):
+            raise RuntimeError("hotcold_kv: hc_prefix_attn_args layout differs between the library and the binding")
         _lib = handle
     return _lib
 
@@ -304,6 +327,15 @@ def step_bind():
                 _bind = mod
             _bind_tried = True
     return _bind
+
+
+def tensor_bind():
+    """The binding module, for the operators that have no other front end."""
+    mod = step_bind()
+    if mod is None:
+        raise RuntimeError(f"hotcold_kv: binding not built ({_BIND_PATH}); "
+                           "run `python hotcold-kv-cache_amd/build_native.py`")
+    return mod
 
 
 class HotColdError(RuntimeError):

@@ -1183,5 +1183,88 @@ def inject_rerope_tab(k_pre, v_staged, cos_t, sin_t, k_dst, v_dst):
     N.check(rc, "hc_inject_rerope_tab")
 
 
+# ---------------------------------------------------------------------------
+# A batch of requests behind one shared prompt: pages and attention
+# ---------------------------------------------------------------------------
+def _stream_of(t):
+    return stream_handle(t.device) if t.is_cuda else 0
+
+
+def extend_pages(lens, new_lens, tables, free_pages, free_count, page_size, num_tokens, lens_out=None,
+                 count_out=None):
+    """Block tables and slot maps of a step, from the requests' lengths.
+
+    lens, new_lens (B,) int32: rows held and rows to come.  tables
+    (B,pages) int32: the pages of each request's rows, in order; the new pages'
+    entries are written.  free_pages (F,) int32, of which the first free_count
+    (1,) int32 are free; pages are taken from the end, for the requests in
+    order.  A request that does not fit (no pages left, a table too short,
+    tokens past num_tokens) keeps its length and gets no slots; requests that
+    need no page are always served.  num_tokens: the rows of the packed token
+    batch (at least the sum of new_lens; the rest is padding).
+
+    Returns (lens (B,), free_count (1,), cu_new (B+1,) int32, slots
+    (num_tokens,), positions (num_tokens,) int64): the new lengths and count
+    (written to lens_out / count_out where given, which may be lens /
+    free_count), the packed batch's offsets, and every token's slot (page *
+    page_size + row) and row in its request, -1 for padding and for requests
+    not served.  Nothing is synchronised: whether all were served is
+    lens_out == lens + new_lens."""
+    *out, rc = N.tensor_bind().extend_pages(lens, new_lens, tables, free_pages, free_count, page_size, num_tokens,
+                                            lens_out, count_out, _stream_of(lens))
+    if rc:
+        N.check(rc, "hc_extend_pages")
+    return tuple(out)
+
+
+def release_pages(lens, keep_lens, tables, free_pages, free_count, page_size, lens_out=None, count_out=None):
+    """Put the pages behind every request's first keep_lens (B,) int32 rows
+    back on the free list (in place): 0 for a finished request, less than its
+    length where tokens were rejected; a request that keeps at least its length
+    is left alone.  The other arguments are extend_pages'.  Returns (lens,
+    free_count), written to lens_out / count_out where given (which may be lens
+    / free_count).  Table entries of released pages stay as they are."""
+    lo, co, rc = N.tensor_bind().release_pages(lens, keep_lens, tables, free_pages, free_count, page_size, lens_out,
+                                               count_out, _stream_of(lens))
+    if rc:
+        N.check(rc, "hc_release_pages")
+    return lo, co
+
+
+def append_paged(slots, k_new, v_new, k_pages, v_pages):
+    """Write rows k_new / v_new (N,Hk,D) or (N,Hk,1,D) into slots (N,) int64 of
+    the pools k_pages / v_pages (pages,Hk,page_size,D): append_rows with a slot
+    map.  Rows whose slot is outside the pool (-1) are skipped; the other slots
+    must be distinct."""
+    rc = N.tensor_bind().append_paged(slots, k_new, v_new, k_pages, v_pages, _stream_of(k_new))
+    if rc:
+        N.check(rc, "hc_append_paged")
+
+
+def prefix_attention(q, k_prefix, v_prefix, k_pages, v_pages, tables, lens, scaling, cu_new=None, max_new=None,
+                     prefix_lens=None, out=None, return_lse=False):
+    """GQA attention of a batch of requests behind one shared prompt.
+
+    q (N,Hq,D) or (N,Hq,1,D): the requests' query tokens, packed; request b has
+    tokens cu_new[b] .. cu_new[b+1] (cu_new (B+1,) int32, with max_new an upper
+    bound on a request's tokens), or one token each without cu_new.  They are
+    the last of its lens[b] own rows, whose keys and values are already in the
+    pools k_pages / v_pages (pages,Hk,page_size,D) at tables (B,pages).  Every
+    token attends the prompt's rows k_prefix / v_prefix (1,Hk,S,D) or (Hk,S,D)
+    -- a hot buffer's, compacted or not; None: no prompt -- and its request's
+    own rows up to itself.  prefix_lens (B,) int32 limits the prompt's rows per
+    request.  The prompt's keys and values are read once for all requests.
+
+    Returns out (N,Hq,D) in q's dtype, with return_lse also the fp32 natural
+    log-sum-exp (N,Hq).  A token that attends nothing gets zeros and -inf.  Rows
+    behind the last request are not written."""
+    o, lse, rc = N.tensor_bind().prefix_attention(q, k_prefix, v_prefix, k_pages, v_pages, tables, lens,
+                                                  scaling, cu_new, max_new, prefix_lens, out, return_lse,
+                                                  _stream_of(q))
+    if rc:
+        N.check(rc, "hc_prefix_attn")
+    return (o, lse) if return_lse else o
+
+
 def default_scaling(head_dim):
     return 1.0 / math.sqrt(head_dim)

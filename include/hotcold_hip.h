@@ -679,6 +679,105 @@ int hc_index_search(int64_t B, int64_t VH, int64_t VD, int64_t cap, const float*
                     uint32_t* keys32, int64_t* hits, int64_t* hits_host, void* wait_event, void* done_event,
                     void* stream);
 
+/*
+ * A batch of requests behind one shared prompt (no counterpart in the
+ * reference, whose caches are one dense tensor per layer with one length for
+ * the whole batch, cache.py:145-148).  The prompt's rows are one dense hot
+ * buffer that every request attends; a request's own rows live in pages of a
+ * pool: k_pages / v_pages [num_pages][Hk][page_size][D], page_size a power of
+ * two.  Row r of request b is in page tables[b*t_sb + r / page_size] at row
+ * r % page_size; its slot is page * page_size + row.  free_pages[0 .. count)
+ * lists the pages nobody holds, taken from its end.
+ *
+ * hc_extend_pages: lens[b] rows are held, new_lens[b] rows come.  Request b
+ * needs the pages of lens + new beyond those of lens; requests that need pages
+ * are served in order while the free list lasts (one that does not fit stops
+ * those behind it; one that needs none is always served).  A request with a
+ * negative length, more pages than table_width, or tokens past num_tokens is
+ * not served and takes nothing.  Writes
+ *   tables     the new pages' entries of the served requests (others stay);
+ *   lens_out   [B] lens + new where served, else lens (may be lens);
+ *   count_out  [1] the free list's new length (may be free_count);
+ *   cu_new     [B+1] sums of max(new_lens, 0), at most num_tokens: request b's
+ *              tokens are cu_new[b] .. cu_new[b+1] of the packed batch;
+ *   slots, positions [num_tokens] int64: each token's slot and row, -1 for
+ *              tokens past the last request or of a request not served.
+ * B <= 4096, num_tokens <= 2^20.
+ */
+int hc_extend_pages(int64_t B, const int32_t* lens, const int32_t* new_lens, int32_t* tables, int64_t t_sb,
+                    int64_t table_width, const int32_t* free_pages, int64_t free_capacity,
+                    const int32_t* free_count, int64_t page_size, int64_t num_tokens, int32_t* lens_out,
+                    int32_t* count_out, int32_t* cu_new, int64_t* slots, int64_t* positions, void* stream);
+
+/*
+ * hc_release_pages: every request keeps its first min(lens, max(keep_lens, 0))
+ * rows (0: a finished request; less than lens: rejected tokens); the pages
+ * behind them are put on the free list, in request and table order.  A request
+ * whose length is negative or past its table is left alone.  lens_out may be
+ * lens, count_out free_count; entries past free_capacity are dropped (the list
+ * was too short for its pool).  Tables are not changed.
+ */
+int hc_release_pages(int64_t B, const int32_t* lens, const int32_t* keep_lens, const int32_t* tables, int64_t t_sb,
+                     int64_t table_width, int32_t* free_pages, int64_t free_capacity, const int32_t* free_count,
+                     int64_t page_size, int32_t* lens_out, int32_t* count_out, void* stream);
+
+/*
+ * hc_append_paged: rows k_new / v_new [N][Hk][D] into their slots of the pool
+ * (hc_append_rows with a slot map).  A slot below 0 or past the pool skips its
+ * row; the others must be distinct.  Rows are multiples of 16 bytes, 16-byte
+ * aligned.
+ */
+int hc_append_paged(int dtype, int64_t N, int64_t Hk, int64_t D, const int64_t* slots,
+                    const void* k_new, int64_t kn_sn, int64_t kn_sh, const void* v_new, int64_t vn_sn, int64_t vn_sh,
+                    void* k_pages, int64_t kg_sp, int64_t kg_sh, int64_t kg_ss,
+                    void* v_pages, int64_t vg_sp, int64_t vg_sh, int64_t vg_ss,
+                    int64_t num_pages, int64_t page_size, void* stream);
+
+/*
+ * hc_prefix_attn: GQA attention of packed query tokens q [N][Hq][D] behind the
+ * shared prompt.  Request b's tokens are cu_new[b] .. cu_new[b+1] (cu_new
+ * NULL: one token a request, N == B), the last of its lens[b] own rows (which
+ * already hold them).  Token i of n attends the prompt's rows
+ * 0 .. prefix_lens[b] (NULL: all prefix_rows) and its own rows
+ * 0 .. lens[b] - n + i, its own row last.  A table entry outside the pool hides its
+ * page's rows.  A token that attends nothing gets zeros (lse -inf).  Rows of
+ * out (and lse) behind the last request are left as they were.
+ *   k_prefix, v_prefix [Hk][prefix_rows][D] (NULL when prefix_rows == 0)
+ *   out [N][Hq][D] in dtype; lse [N][Hq] fp32 (may be NULL): the natural
+ *     logarithm of the softmax's sum of exponentials.
+ *   max_new: an upper bound on a request's tokens (1 without cu_new).  Tokens
+ *     of a request beyond it are not computed.
+ *   D 16, 32, 64 or 128.  Every stride and pointer is a multiple of 16 bytes.
+ *   The workspace holds hc_prefix_attn_workspace_size(args) bytes (a negative
+ *   value: the arguments are refused, as hc_prefix_attn does), needs no
+ *   initialisation and is in use until the stream reaches the end of the call.
+ * Every field is 8 bytes, so the layout has no padding;
+ * hc_prefix_attn_args_size() returns sizeof for a binding to check.
+ */
+typedef struct hc_prefix_attn_args {
+  int64_t dtype, N, B, Hq, Hk, D;
+  const void* q; int64_t q_sn, q_sh;
+  const void* k_prefix; int64_t kp_sh, kp_ss;
+  const void* v_prefix; int64_t vp_sh, vp_ss;
+  int64_t prefix_rows;
+  const int32_t* prefix_lens;
+  const void* k_pages; int64_t kg_sp, kg_sh, kg_ss;
+  const void* v_pages; int64_t vg_sp, vg_sh, vg_ss;
+  int64_t num_pages, page_size;
+  const int32_t* tables; int64_t t_sb, table_width;
+  const int32_t* lens;
+  const int32_t* cu_new;
+  int64_t max_new;
+  double scaling;
+  void* out; int64_t o_sn, o_sh;
+  float* lse; int64_t l_sn, l_sh;
+  void* workspace; int64_t workspace_bytes;
+} hc_prefix_attn_args;
+
+int64_t hc_prefix_attn_workspace_size(const hc_prefix_attn_args* args);
+int hc_prefix_attn(const hc_prefix_attn_args* args, void* stream);
+int64_t hc_prefix_attn_args_size(void);
+
 #ifdef __cplusplus
 }
 #endif
