@@ -1,117 +1,60 @@
 // Attention of a batch behind one shared prompt: host side and C ABI.
 #include <algorithm>
+#include <cmath>
 
-#include "hc_common.h"
+#include "hc_prefix_kernels.h"
 
 namespace hc {
 
 int page_shift(int64_t P);   // hc_pages.hip
 
-struct PrefixArgs {
-  const void* q;
-  int64_t q_sn, q_sh;
-  const void* kp;
-  int64_t kp_sh, kp_ss;
-  const void* vp;
-  int64_t vp_sh, vp_ss;
-  const int32_t* prefix_lens;
-  const void* kg;
-  int64_t kg_sp, kg_sh, kg_ss;
-  const void* vg;
-  int64_t vg_sp, vg_sh, vg_ss;
-  const int32_t* tables;
-  int64_t t_sb;
-  const int32_t* lens;
-  const int32_t* cu;
-  void* out;
-  int64_t o_sn, o_sh;
-  float* lse;
-  int64_t l_sn, l_sh;
-  int64_t num_pages;
-  float scaling;
-  int N, B, G, D, S, T, lp;
+extern template void launch_prefix<half_t>(const PrefixArgs&, int64_t, hipStream_t);
+extern template void launch_prefix<bf16_t>(const PrefixArgs&, int64_t, hipStream_t);
+extern template void launch_prefix<float>(const PrefixArgs&, int64_t, hipStream_t);
+
+constexpr int kCus = 256;
+
+// How a call is laid out over workgroups.
+struct PrefixPlan {
+  int p_wr, p_tiles, p_splits, p_chunk, o_wr, o_tiles, o_splits, m_tiles;
+  int64_t items, slots;
 };
 
-// One workgroup per (token, query head): 256 keys at a time, a thread per
-// key, then a thread per (dimension, part of the keys).
-template <typename T>
-__global__ __launch_bounds__(256) void prefix_attn_kernel(PrefixArgs a) {
-  __shared__ float s_q[128], s_p[256], s_red[8], s_acc[256];
-  __shared__ int64_t s_voff[256];
-  const int n = blockIdx.x, h = blockIdx.y, hk = h / a.G, tid = threadIdx.x;
-  int b = n, c1 = n + 1;
-  if (a.cu) {
-    if (n >= min(a.cu[a.B], a.N)) return;
-    int lo = 0, hi = a.B - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (a.cu[mid] <= n) lo = mid; else hi = mid - 1;
-    }
-    b = lo;
-    c1 = a.cu[lo + 1];
-  }
-  const int S = a.prefix_lens ? min(max(a.prefix_lens[b], 0), a.S) : a.S;
-  const int len = min(max(a.lens[b], 0), a.T << a.lp);
-  const int own = max(0, len - (c1 - 1 - n));
-  const T* q = (const T*)a.q + n * a.q_sn + h * a.q_sh;
-  for (int d = tid; d < a.D; d += 256) s_q[d] = to_f32(q[d]) * a.scaling;
-  const int parts = 256 / a.D, d = tid % a.D, part = tid / a.D;
-  float m = -INFINITY, l = 0.f, acc = 0.f;
-  for (int64_t k0 = 0; k0 < (int64_t)S + own; k0 += 256) {
-    __syncthreads();
-    const int64_t key = k0 + tid;
-    float x = -INFINITY;
-    int64_t voff = -1;
-    const T* kr = nullptr;
-    if (key < S) {
-      kr = (const T*)a.kp + hk * a.kp_sh + key * a.kp_ss;
-      voff = hk * a.vp_sh + key * a.vp_ss;
-    } else if (key < (int64_t)S + own) {
-      const int r = (int)(key - S);
-      const int64_t page = a.tables[b * a.t_sb + (r >> a.lp)];
-      const int row = r & ((1 << a.lp) - 1);
-      if (page >= 0 && page < a.num_pages) {
-        kr = (const T*)a.kg + page * a.kg_sp + hk * a.kg_sh + row * a.kg_ss;
-        voff = page * a.vg_sp + hk * a.vg_sh + row * a.vg_ss;
+// Waves that share keys: as many as 32 rows each fill.
+int rows_waves(int64_t rows, int waves) {
+  int wr = 1;
+  while (wr < waves && rows > 32 * wr) wr *= 2;
+  return wr;
+}
+
+PrefixPlan plan_prefix(const hc_prefix_attn_args* x) {
+  PrefixPlan p{};
+  const int waves = x->D * dtype_size((int)x->dtype) >= 512 ? 4 : 8;
+  const int64_t G = x->Hq / x->Hk, rows = x->N * G, most = std::min(x->max_new, x->N);
+  if (x->prefix_rows > 0) {
+    p.p_wr = rows_waves(rows, waves);
+    p.p_tiles = (int)cdiv(rows, 32 * p.p_wr);
+    const int64_t bn = p.p_wr == waves ? 64 : 32 * (waves / p.p_wr), units = p.p_tiles * x->Hk;
+    // the fewest rounds of workgroups times a workgroup's keys and fixed cost
+    int64_t best = INT64_MAX;
+    for (int64_t s = 1; s <= 256 && s <= cdiv(x->prefix_rows, bn); ++s) {
+      const int64_t chunk = cdiv(cdiv(x->prefix_rows, s), bn) * bn, splits = cdiv(x->prefix_rows, chunk);
+      const int64_t cost = cdiv(units * splits, (int64_t)kCus) * (chunk + 256);
+      if (cost < best) {
+        best = cost;
+        p.p_splits = (int)splits;
+        p.p_chunk = (int)chunk;
       }
     }
-    if (kr) {
-      x = 0.f;
-      for (int i = 0; i < a.D; ++i) x += s_q[i] * to_f32(kr[i]);
-    }
-    s_voff[tid] = voff;
-    float t = wave_max(x);
-    if ((tid & 63) == 0) s_red[tid >> 6] = t;
-    __syncthreads();
-    t = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-    const float mn = fmaxf(m, t);
-    const float p = kr ? expf(x - mn) : 0.f;
-    s_p[tid] = p;
-    t = wave_sum(p);
-    if ((tid & 63) == 0) s_red[4 + (tid >> 6)] = t;
-    __syncthreads();
-    const float alpha = mn == -INFINITY ? 1.f : expf(m - mn);
-    l = l * alpha + (s_red[4] + s_red[5] + s_red[6] + s_red[7]);
-    acc *= alpha;
-    m = mn;
-    if (part < parts)
-      for (int j = part; j < 256; j += parts) {
-        const int64_t v = s_voff[j];
-        if (v >= 0) {
-          const T* base = k0 + j < S ? (const T*)a.vp : (const T*)a.vg;
-          acc += s_p[j] * to_f32(base[v + d]);
-        }
-      }
   }
-  __syncthreads();
-  s_acc[tid] = acc;
-  __syncthreads();
-  if (tid < a.D) {
-    float t = 0.f;
-    for (int j = 0; j < parts; ++j) t += s_acc[j * a.D + tid];
-    ((T*)a.out)[n * a.o_sn + h * a.o_sh + tid] = from_f32<T>(l == 0.f ? 0.f : t / l);
-  }
-  if (tid == 0 && a.lse) a.lse[n * a.l_sn + h * a.l_sh] = l == 0.f ? -INFINITY : m + logf(l);
+  p.o_wr = rows_waves(most * G, waves);
+  p.o_tiles = (int)cdiv(most * G, 32 * p.o_wr);
+  const int64_t units = x->B * x->Hk * p.o_tiles, longest = x->table_width * x->page_size;
+  p.o_splits = (int)std::max<int64_t>(1, std::min<int64_t>({cdiv((int64_t)(4 * kCus), units), cdiv(longest, (int64_t)256), 64}));
+  p.m_tiles = (int)cdiv(most * x->Hq * (x->D / 4), (int64_t)256);
+  p.items = (int64_t)p.p_tiles * x->Hk * p.p_splits + units * p.o_splits;
+  p.slots = p.p_splits + p.o_splits;
+  return p;
 }
 
 }  // namespace hc
@@ -144,7 +87,8 @@ static int check_args(const hc_prefix_attn_args* x) {
              (long long)x->page_size, (long long)x->t_sb);
   HC_REQUIRE(x->cu_new || x->N == x->B, "prefix_attention: without cu_new every request has one token (N=%lld, B=%lld)",
              (long long)x->N, (long long)x->B);
-  HC_REQUIRE(x->max_new >= 1 && (x->cu_new || x->max_new == 1), "prefix_attention: max_new=%lld", (long long)x->max_new);
+  HC_REQUIRE(x->max_new >= 1 && x->max_new <= (1 << 20) && (x->cu_new || x->max_new == 1),
+             "prefix_attention: max_new=%lld", (long long)x->max_new);
   HC_REQUIRE(x->N == 0 || (x->q && x->out && x->k_pages && x->v_pages && x->tables && x->lens &&
                  (x->prefix_rows == 0 || (x->k_prefix && x->v_prefix))),
              "prefix_attention: null pointer");
@@ -154,34 +98,59 @@ static int check_args(const hc_prefix_attn_args* x) {
   const int64_t st[] = {x->q_sn, x->q_sh, x->kp_sh, x->kp_ss, x->vp_sh, x->vp_ss, x->kg_sp, x->kg_sh, x->kg_ss,
                         x->vg_sp, x->vg_sh, x->vg_ss, x->o_sn, x->o_sh};
   for (const int64_t s : st)
-    HC_REQUIRE((s * es) % 16 == 0, "prefix_attention: strides must be multiples of 16 bytes (got %lld elements)",
+    HC_REQUIRE(s >= 0 && (s * es) % 16 == 0, "prefix_attention: strides must be whole multiples of 16 bytes (got %lld elements)",
                (long long)s);
+  // (a load addresses its rows by 32-bit offsets from the first)
+  HC_REQUIRE(std::max({x->kp_ss, x->vp_ss, x->kg_ss, x->vg_ss}) * es <= (1 << 25),
+             "prefix_attention: key and value rows more than 32 MiB apart");
   return HC_OK;
 }
 
-extern "C" int64_t hc_prefix_attn_workspace_size(const hc_prefix_attn_args* x) { return check_args(x); }
+extern "C" int64_t hc_prefix_attn_workspace_size(const hc_prefix_attn_args* x) {
+  if (const int rc = check_args(x)) return rc;
+  if (x->N == 0) return 0;
+  return (plan_prefix(x).slots * x->N * x->Hq * (x->D + 2) + 4) * 4;
+}
 
 extern "C" int hc_prefix_attn(const hc_prefix_attn_args* x, void* stream) {
   if (const int rc = check_args(x)) return rc;
   if (x->N == 0) return HC_OK;
-  const int dtype = (int)x->dtype, lp = page_shift(x->page_size);
+  const int64_t need = hc_prefix_attn_workspace_size(x);
+  if (!x->workspace || x->workspace_bytes < need)
+    return set_error(HC_ERR_WORKSPACE, "prefix_attention: workspace of %lld bytes, %lld needed",
+                     (long long)(x->workspace ? x->workspace_bytes : 0), (long long)need);
+  HC_REQUIRE((uintptr_t)x->workspace % 16 == 0, "prefix_attention: the workspace must be 16-byte aligned");
+  const PrefixPlan p = plan_prefix(x);
+  HC_REQUIRE(p.items <= INT32_MAX && x->B * p.m_tiles <= INT32_MAX, "prefix_attention: %lld workgroups",
+             (long long)p.items);
+  const int dtype = (int)x->dtype;
+  const int64_t es = dtype_size(dtype);
   PrefixArgs a{};
-  a.q = x->q; a.q_sn = x->q_sn; a.q_sh = x->q_sh;
-  a.kp = x->k_prefix; a.kp_sh = x->kp_sh; a.kp_ss = x->kp_ss;
-  a.vp = x->v_prefix; a.vp_sh = x->vp_sh; a.vp_ss = x->vp_ss;
+  a.q = (const char*)x->q; a.q_sn = x->q_sn * es; a.q_sh = x->q_sh * es;
+  a.kp = (const char*)x->k_prefix; a.kp_sh = x->kp_sh * es; a.kp_ss = x->kp_ss * es;
+  a.vp = (const char*)x->v_prefix; a.vp_sh = x->vp_sh * es; a.vp_ss = x->vp_ss * es;
+  a.kg = (const char*)x->k_pages; a.kg_sp = x->kg_sp * es; a.kg_sh = x->kg_sh * es; a.kg_ss = x->kg_ss * es;
+  a.vg = (const char*)x->v_pages; a.vg_sp = x->vg_sp * es; a.vg_sh = x->vg_sh * es; a.vg_ss = x->vg_ss * es;
   a.prefix_lens = x->prefix_lens;
-  a.kg = x->k_pages; a.kg_sp = x->kg_sp; a.kg_sh = x->kg_sh; a.kg_ss = x->kg_ss;
-  a.vg = x->v_pages; a.vg_sp = x->vg_sp; a.vg_sh = x->vg_sh; a.vg_ss = x->vg_ss;
   a.tables = x->tables; a.t_sb = x->t_sb; a.lens = x->lens; a.cu = x->cu_new;
-  a.out = x->out; a.o_sn = x->o_sn; a.o_sh = x->o_sh;
+  a.out = (char*)x->out; a.o_sn = x->o_sn * es; a.o_sh = x->o_sh * es;
   a.lse = x->lse; a.l_sn = x->l_sn; a.l_sh = x->l_sh;
-  a.num_pages = x->num_pages; a.scaling = (float)x->scaling;
-  a.N = (int)x->N; a.B = (int)x->B; a.G = (int)(x->Hq / x->Hk); a.D = (int)x->D; a.S = (int)x->prefix_rows;
-  a.T = (int)x->table_width; a.lp = lp;
-  const dim3 grid((unsigned)x->N, (unsigned)x->Hq);
+  a.part_ml = (float*)x->workspace;
+  a.part_o = a.part_ml + (p.slots * x->N * x->Hq * 2 + 3) / 4 * 4;
+  const float scale = (float)(std::fabs(x->scaling) * 1.4426950408889634);
+  a.scale_log2 = scale == 0.f ? 1.f : scale;
+  a.q_and = scale == 0.f ? 0u : ~0u;
+  a.q_xor = scale == 0.f || !std::signbit(x->scaling) ? 0u : dtype == HC_DTYPE_F32 ? 0x80000000u : 0x80008000u;
+  a.N = (int)x->N; a.B = (int)x->B; a.Hq = (int)x->Hq; a.Hk = (int)x->Hk; a.G = (int)(x->Hq / x->Hk);
+  a.D = (int)x->D; a.S = (int)x->prefix_rows; a.T = (int)x->table_width; a.lp = page_shift(x->page_size);
+  a.num_pages = (int)x->num_pages;
+  a.max_new = (int)std::min<int64_t>(x->max_new, x->N);
+  a.p_wr = p.p_wr; a.p_tiles = p.p_tiles; a.p_splits = p.p_splits; a.p_chunk = p.p_chunk;
+  a.p_items = p.p_tiles * a.Hk * p.p_splits;
+  a.o_wr = p.o_wr; a.o_tiles = p.o_tiles; a.o_splits = p.o_splits; a.m_tiles = p.m_tiles;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (dtype == HC_DTYPE_F16) prefix_attn_kernel<half_t><<<grid, 256, 0, s>>>(a);
-  else if (dtype == HC_DTYPE_BF16) prefix_attn_kernel<bf16_t><<<grid, 256, 0, s>>>(a);
-  else prefix_attn_kernel<float><<<grid, 256, 0, s>>>(a);
+  if (dtype == HC_DTYPE_F16) launch_prefix<half_t>(a, p.items, s);
+  else if (dtype == HC_DTYPE_BF16) launch_prefix<bf16_t>(a, p.items, s);
+  else launch_prefix<float>(a, p.items, s);
   return check_launch("prefix_attention");
 }

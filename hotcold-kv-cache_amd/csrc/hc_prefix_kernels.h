@@ -1,0 +1,750 @@
+// Device side of the attention behind a shared prompt (hc_prefix.hip holds the
+// host side and the C ABI; the kernels are instantiated once per element type
+// in hc_prefix_{f16,bf16,f32}.hip, so the three compile in parallel).
+//
+// Query token i of request b (n tokens, len own rows) attends the prompt's
+// rows [0, prefix_lens[b]) and its own rows [0, len - n + i].  With G query
+// heads per KV head, the batch is N * G query rows per KV head.
+//
+// One launch has two kinds of items, each one workgroup:
+//   * prompt items: (KV head, tile of query rows packed over all requests, key
+//     range of the prompt): the prompt is read once per tile, for all requests;
+//   * own items: (request, KV head, tile of its query rows, key range of its
+//     pages).
+// Each writes (max, sum, unnormalised output) of its rows for its keys, and a
+// second launch joins them.
+//
+// A workgroup's NW waves are WR x WK: WR waves share the keys and take 32
+// query rows each, WK waves take different keys.  WR follows the rows there
+// are (32 to 32 NW a tile): a single request's few rows put every wave on keys
+// of its own.
+//   * Scores are K.Q^T (v_mfma_f32_32x32x16, fp32 inputs 32x32x2): a lane
+//     holds one query row's scores of 16 keys, so the row's running max and
+//     sum live in its two lanes, and its probabilities are, as they stand, the
+//     B operand of V^T.P^T: the product's order of keys is the score layout's
+//     (key (i & 3) + 8 (i / 4) + 4 (lane / 32) in register i), and V^T's
+//     operand is read in that order, by LDS transpose reads (ds_read_b64_tr)
+//     for 2-byte types.  The output is transposed, too: a lane owns its
+//     query's column, and the rescale is a multiply by the lane's own factor.
+//   * K and V tiles go to LDS by asynchronous loads (global_load_lds_dwordx4)
+//     with a 16-byte piece p of row r stored at p ^ f(r): f spreads 16 rows'
+//     same piece over all banks (K's operand reads) and 4 rows' piece pairs
+//     over distinct ones (V's transpose reads).
+//   * Softmax is online, in fp32 and the log2 domain, with a lazy reference
+//     (kLazy): the accumulators are rescaled only where a row's max passes its
+//     reference by 2^8.  Probabilities are rounded once to the inputs' 2-byte
+//     type (fp32: not at all); their sum takes them unrounded.
+//   * Tiles that every row of the wave sees whole take no masks.  Others
+//     select per key; rows no request holds, or in pages outside the pool, are
+//     zeroed in LDS first, so that nothing stale enters a product.  Where rows
+//     of one tile see different keys and a value is not finite, the tile's
+//     product is taken key by key (0 times infinity must not reach a row that
+//     does not attend it).
+#pragma once
+#include "hc_common.h"
+
+namespace hc {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+
+struct PrefixArgs {
+  const char* q;   // strides in bytes
+  int64_t q_sn, q_sh;
+  const char* kp;
+  int64_t kp_sh, kp_ss;
+  const char* vp;
+  int64_t vp_sh, vp_ss;
+  const char* kg;
+  int64_t kg_sp, kg_sh, kg_ss;
+  const char* vg;
+  int64_t vg_sp, vg_sh, vg_ss;
+  const int32_t* prefix_lens;
+  const int32_t* tables;
+  int64_t t_sb;
+  const int32_t* lens;
+  const int32_t* cu;
+  char* out;
+  int64_t o_sn, o_sh;
+  float* lse;
+  int64_t l_sn, l_sh;
+  float* part_o;   // [slots][N * Hq][D]
+  float* part_ml;  // [slots][N * Hq][2]
+  // |scaling| log2(e), its sign and zero moved to q: (q & q_and) ^ q_xor.  (A
+  // scale of 0 would turn masked scores, -inf, into NaN.)
+  float scale_log2;
+  uint32_t q_and, q_xor;
+  int N, B, Hq, Hk, G, D, S, T, lp, num_pages, max_new;
+  // prompt items: WR of their workgroups, row tiles, key splits and rows a
+  // split; own items: WR, row tiles and splits of one request
+  int p_wr, p_tiles, p_splits, p_chunk, p_items;
+  int o_wr, o_tiles, o_splits;
+  // merge: tiles of rows of one request
+  int m_tiles;
+};
+
+constexpr float kLazy = 8.f;
+constexpr int kPageIds = 2048;  // page numbers held in LDS at a time
+
+template <typename T, int D>
+struct PrefixShape {
+  static constexpr int kRowB = D * (int)sizeof(T);
+  static constexpr int kWaves = kRowB >= 512 ? 4 : 8;  // K and V of 32 keys a wave fit LDS
+  static constexpr int kPieces = kRowB / 16;
+  static constexpr int kTileB = kWaves * 32 * 2 * kRowB;   // WR = 1: one buffer; WR >= 2: two of BN keys
+  static constexpr int kOutB = kWaves * 32 * (D + 4) * 4;  // the outputs of all waves
+  static constexpr int kLds = kTileB > kOutB ? kTileB : kOutB;
+};
+
+// Rows of own keys per split of a request with len rows.
+__host__ __device__ __forceinline__ int own_chunk(int len, int splits) {
+  const int c = (len + splits - 1) / splits;
+  return max((c + 255) / 256 * 256, 256);
+}
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// max / sum of a lane's value with lane ^ 32's
+__device__ __forceinline__ float half_max(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// 16 bytes per lane from p (the lane's own) to LDS at byte offset lds (the
+// wave's) + 16 * lane, asynchronously: complete after vm_wait.  The compiler
+// does not see the write; every use is behind a vm_wait, which it does not
+// move memory accesses across.
+__device__ __forceinline__ void load_to_lds(const void* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
+}
+// ... from the wave's address base plus the lane's offset.  (The base may come
+// from a v_readfirstlane, which takes five wait states before a memory
+// instruction may read it; the compiler's own count does not look into asm.)
+__device__ __forceinline__ void load_to_lds(const void* base, uint32_t off, uint32_t lds) {
+  const uint64_t at = (uint64_t)base;
+  const uint64_t s = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32 |
+                     (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(s)
+               : "memory");
+}
+__device__ __forceinline__ void lds_wait() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void vm_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// The lane's value again, as one the compiler does not know: what is computed
+// from it in a rare path stays there, instead of in registers of the whole loop.
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<half_t> {
+  typedef half8 frag;
+  __device__ static floatx16 mma(half8 a, half8 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<bf16_t> {
+  typedef bf16x8 frag;
+  __device__ static floatx16 mma(bf16x8 a, bf16x8 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<float> {
+  typedef floatx4 frag;
+};
+
+// What an item's workgroup works on.
+struct Item {
+  int hk, tok0, row0, rows;   // query rows [row0, rows) of tokens tok0 + row / G
+  int kbeg, kend;             // keys
+  int lim0, cut;              // own items: row r sees keys below lim0 + r / G (at least 0)
+  const int32_t* table;       // own items: the request's pages
+  int slot;                   // where its partial goes
+};
+
+template <typename T, int D, int WR, bool kOwn>
+__device__ __forceinline__ void prefix_item(const PrefixArgs& a, const Item& it, char* smem, int32_t* s_pid, float* s_ml) {
+  using Sh = PrefixShape<T, D>;
+  constexpr int kRowB = Sh::kRowB, kPieces = Sh::kPieces, WK = Sh::kWaves / WR;
+  constexpr int KT = WK == 1 ? 64 : 32;        // keys a wave takes of a tile
+  constexpr int KB = KT / 32, BN = WK * KT;
+  constexpr int kStages = WR == 1 ? 1 : 2;
+  constexpr int kRows = KT / WR;               // rows of a tile a wave loads
+  constexpr int kPerLoad = 64 / kPieces;       // rows of one load
+  constexpr int kLoads = (kRows + kPerLoad - 1) / kPerLoad;
+  constexpr bool kPartial = kRows < kPerLoad;  // a load's last lanes stay idle
+  constexpr int kSt = BN * kRowB;              // bytes of a tile's K, or V
+  static_assert(2 * kSt * kStages <= Sh::kLds, "tiles fit LDS");
+  constexpr int NB = (D + 31) / 32;            // blocks of 32 output dimensions
+  constexpr bool kF32 = sizeof(T) == 4;
+  constexpr int NQ = kF32 ? D / 8 : (D + 15) / 16;
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int wr = wave % WR, wk = wave / WR;
+  const int col = lane & 31, half = lane >> 5;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+
+  // ---- the wave's query rows
+  const int r = it.row0 + 32 * wr + col;
+  const bool live = r < it.rows;
+  const int tok = it.tok0 + (live ? r / a.G : 0);
+  const int head = it.hk * a.G + (live ? r % a.G : 0);
+  typename Mma<T>::frag qf[NQ];
+  {
+    const char* qp = a.q + tok * a.q_sn + head * a.q_sh;
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) {
+      u32x4 x = {0u, 0u, 0u, 0u};
+      if (live) x = ld16(qp + 32 * t + 16 * half);
+      x = (x & a.q_and) ^ a.q_xor;
+      qf[t] = __builtin_bit_cast(typename Mma<T>::frag, x);
+    }
+  }
+  int lim = it.kend;
+  if constexpr (kOwn) {
+    if (live) lim = min(lim, max(0, it.lim0 + r / a.G));
+  } else {
+    if (live && a.prefix_lens) {
+      int b = tok;
+      if (a.cu) {   // the last request that starts at or before the token
+        int lo = 0, hi = a.B - 1;
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (a.cu[mid] <= tok) lo = mid; else hi = mid - 1;
+        }
+        b = lo;
+      }
+      lim = min(lim, max(0, a.prefix_lens[b]));
+    }
+  }
+  // keys every row of the workgroup sees, and keys some row sees
+  int all = it.kend, kend = it.kend;
+  if constexpr (kOwn) {
+    all = min(it.kend, max(0, it.lim0 + it.row0 / a.G));   // (the first row sees least; kend is the last's)
+  } else if (a.prefix_lens) {
+    int lo = lim, hi = live ? lim : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      lo = min(lo, __shfl_xor(lo, o, 64));
+      hi = max(hi, __shfl_xor(hi, o, 64));
+    }
+    int* s_lim = reinterpret_cast<int*>(s_ml);
+    if (lane == 0) {
+      s_lim[wave] = lo;
+      s_lim[Sh::kWaves + wave] = hi;
+    }
+    __syncthreads();
+    kend = 0;
+#pragma unroll
+    for (int w = 0; w < Sh::kWaves; ++w) {
+      all = min(all, s_lim[w]);
+      kend = max(kend, s_lim[Sh::kWaves + w]);
+    }
+    all = __builtin_amdgcn_readfirstlane(all);
+    kend = __builtin_amdgcn_readfirstlane(kend);
+    __syncthreads();
+  }
+  // rows see different keys: a value that is not finite may have to reach some
+  // of them only
+  const bool ragged = all != kend;
+
+  floatx16 acc[NB];
+#pragma unroll
+  for (int d = 0; d < NB; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+
+  const char* kbase = kOwn ? a.kg + it.hk * a.kg_sh : a.kp + it.hk * a.kp_sh;
+  const char* vbase = kOwn ? a.vg + it.hk * a.vg_sh : a.vp + it.hk * a.vp_sh;
+  // (a segment's first page may be entered in its middle)
+  const int seg_keys = kOwn ? ((kPageIds - 1) << min(a.lp, 12)) / BN * BN : 0x7fffffff;
+
+  // f(r) of row r: pieces of 16 rows with the same number lie on distinct
+  // 16-byte columns of the 256 bytes all banks hold, pairs of 4 rows too
+  constexpr int kXor = kPieces < 16 ? kPieces : 16;
+  constexpr int kXorBits = kXor == 16 ? 4 : kXor == 8 ? 3 : kXor == 4 ? 2 : 1;
+  constexpr int kRows256 = 16 / kXor;
+  auto swz = [](int row) {
+    const int x = (row / kRows256) & (kXor - 1);
+    return ((x << 1) | (x >> (kXorBits - 1))) & (kXor - 1);
+  };
+
+  for (int seg = it.kbeg, send; seg < kend; seg = send) {
+    send = kend - seg > seg_keys ? seg + seg_keys : kend;
+    bool bad_pages = false;
+    const int page0 = seg >> a.lp;
+    if constexpr (kOwn) {
+      // (the barrier also keeps the last segment's tiles until all are read)
+      __syncthreads();
+      int bad = 0;
+      const int n = ((send - 1) >> a.lp) - page0 + 1;
+      for (int i = threadIdx.x; i < n; i += Sh::kWaves * 64) {
+        const int p = it.table[page0 + i];
+        const bool ok = (uint32_t)p < (uint32_t)a.num_pages;
+        s_pid[i] = ok ? p : -1;
+        bad |= !ok;
+      }
+      bad_pages = __builtin_amdgcn_readfirstlane(__syncthreads_or(bad)) != 0;
+    }
+
+    // asynchronous loads of the wave's rows of the tile at key0; a load's rows
+    // are consecutive keys: of one page where pages hold that many
+    auto issue = [&](int key0, int stage, bool v) {
+      const int piece = lane % kPieces, sub = lane / kPieces;
+      const uint32_t dst = lds0 + (uint32_t)((stage * 2 + (v ? 1 : 0)) * kSt + (wk * KT + wr * kRows) * kRowB);
+      const int64_t ss = kOwn ? (v ? a.vg_ss : a.kg_ss) : (v ? a.vp_ss : a.kp_ss);
+      const char* base = v ? vbase : kbase;
+      const int first = key0 + wk * KT + wr * kRows;
+      const bool whole = first + kRows <= send && (!kOwn || (1 << a.lp) >= kPerLoad);
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const uint32_t d = __builtin_amdgcn_readfirstlane(dst + (uint32_t)(j * 1024));
+        const int at = 16 * (piece ^ swz(wr * kRows + j * kPerLoad + sub));
+        if (whole) {
+          const int key = first + j * kPerLoad;
+          const char* p = base;
+          if constexpr (kOwn) {
+            const int pid = __builtin_amdgcn_readfirstlane(s_pid[(key >> a.lp) - page0]);
+            p += (int64_t)max(pid, 0) * (v ? a.vg_sp : a.kg_sp) + (int64_t)(key & ((1 << a.lp) - 1)) * ss;
+          } else {
+            p += (int64_t)key * ss;
+          }
+          if (!kPartial || lane < kRows * kPieces) load_to_lds(p, (uint32_t)sub * (uint32_t)ss + (uint32_t)at, d);
+        } else {
+          // keys past the end load the last one's row (zeroed below)
+          const int key = min(first + j * kPerLoad + sub, send - 1);
+          const char* p = base;
+          if constexpr (kOwn) {
+            const int pid = max(s_pid[(key >> a.lp) - page0], 0);
+            p += (int64_t)pid * (v ? a.vg_sp : a.kg_sp) + (int64_t)(key & ((1 << a.lp) - 1)) * ss;
+          } else {
+            p += (int64_t)key * ss;
+          }
+          if (!kPartial || lane < kRows * kPieces) load_to_lds(p + at, d);
+        }
+      }
+    };
+    auto hidden = [&](int key) {   // a key of the segment's tiles that nobody attends
+      if (key >= send) return true;
+      if constexpr (kOwn) return bad_pages && s_pid[(key >> a.lp) - page0] < 0;
+      return false;
+    };
+    // zero the wave's loaded rows of keys nobody attends
+    auto clear = [&](int key0, int stage, bool v) {
+      const int ln = fresh(lane);
+#pragma unroll 1
+      for (int j = 0; j < kLoads; ++j) {
+        const int row = wr * kRows + j * kPerLoad + ln / kPieces;
+        if ((!kPartial || ln < kRows * kPieces) && hidden(key0 + wk * KT + row))
+          st16(smem + (stage * 2 + (v ? 1 : 0)) * kSt + (wk * KT + row) * kRowB + (ln % kPieces) * 16,
+               u32x4{0u, 0u, 0u, 0u});
+      }
+    };
+
+    issue(seg, 0, false);
+    issue(seg, 0, true);
+    // one tile; kAll: every row sees all of its keys
+    auto do_tile = [&](int tile, int n, auto all_see) {
+      constexpr bool kAll = decltype(all_see)::value;
+      const int stage = kStages == 1 ? 0 : (n & 1);
+      const bool more = tile + BN < send;
+      const bool edge = !kAll && (tile + BN > send || bad_pages);
+      if constexpr (WR == 1) {
+        // the wave's own rows: its V loads (kLoads of them) may be in flight
+        vm_wait<kLoads>();
+        if (edge) clear(tile, 0, false);
+      } else {
+        vm_wait<0>();
+        if (edge) {
+          clear(tile, stage, false);
+          clear(tile, stage, true);
+        }
+        __syncthreads();
+        if (more) {
+          issue(tile + BN, stage ^ 1, false);
+          issue(tile + BN, stage ^ 1, true);
+        }
+      }
+      const char* ks = smem + stage * 2 * kSt + wk * KT * kRowB;
+      const char* vs = ks + kSt;
+      const int key0 = tile + wk * KT;
+
+      // ---- scores
+      floatx16 s[KB];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
+#pragma unroll
+      for (int t = 0; t < NQ; ++t)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          const int row = 32 * kb + col;
+          const u32x4 x = ld16(ks + row * kRowB + (((2 * t + half) ^ swz(row)) << 4));
+          if constexpr (kF32) {
+            const floatx4 f = __builtin_bit_cast(floatx4, x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(f[j], qf[t][j], s[kb], 0, 0, 0);
+          } else {
+            s[kb] = Mma<T>::mma(__builtin_bit_cast(typename Mma<T>::frag, x), qf[t], s[kb]);
+          }
+        }
+      if constexpr (WR == 1) {
+        if (more) {
+          lds_wait();   // the tile's reads are done
+          issue(tile + BN, 0, false);
+        }
+      }
+
+      __builtin_amdgcn_sched_barrier(0);
+      // ---- softmax
+      if constexpr (!kAll) {
+        const int first = key0 + 4 * fresh(half);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int key = first + 32 * kb + (i & 3) + 8 * (i >> 2);
+            bool see = key < lim;
+            if (bad_pages) see = see && !hidden(key);
+            s[kb][i] = see ? s[kb][i] : -INFINITY;
+          }
+      }
+      float t = s[0][0];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t = fmaxf(t, s[kb][i]);
+      t = half_max(t) * a.scale_log2;
+      const bool bump = t > m + kLazy;
+      if (__any(bump)) {
+        const float mn = bump ? t : m;
+        const float alpha = bump ? exp2_hw(m - mn) : 1.f;
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < NB; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
+      }
+      const float ref = m == -INFINITY ? 0.f : m;   // (a row that has seen nothing yet: its terms are 0)
+      float sum = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          s[kb][i] = exp2_hw(__builtin_fmaf(s[kb][i], a.scale_log2, -ref));
+          sum += s[kb][i];
+        }
+      l += sum;
+      if constexpr (WR == 1) {
+        if (more) vm_wait<kLoads>(); else vm_wait<0>();
+        if (edge) clear(tile, 0, true);
+      }
+
+      __builtin_amdgcn_sched_barrier(0);
+      // ---- output
+      bool slow = false;
+      if (!kAll && ragged) {
+        // a value that is not finite in this tile?
+        uint32_t odd = 0;
+        for (int i = fresh(lane); i < KT * kPieces; i += 64) {
+          const u32x4 x = ld16(vs + 16 * i);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            if constexpr (kF32) {
+              odd |= (x[w] & 0x7f800000u) == 0x7f800000u;
+            } else {
+              constexpr uint32_t kExp = std::is_same<T, half_t>::value ? 0x7c00u : 0x7f80u;
+              odd |= (x[w] & kExp) == kExp;
+              odd |= ((x[w] >> 16) & kExp) == kExp;
+            }
+          }
+        }
+        slow = __any(odd);
+      }
+      // (with slow the product is taken of zeros)
+      if constexpr (kF32) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int row = 32 * kb + (i & 3) + 8 * (i >> 2) + 4 * half;
+#pragma unroll
+            for (int d = 0; d < NB; ++d) {
+              const int dim = min(32 * d + col, D - 1);   // (outputs past D are not used)
+              float v = *reinterpret_cast<const float*>(vs + row * kRowB + (((dim >> 2) ^ swz(row)) << 4) + (dim & 3) * 4);
+              float p = s[kb][i];
+              if constexpr (!kAll) {
+                v = slow ? 0.f : v;
+                p = slow ? 0.f : p;
+              }
+              acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p, acc[d], 0, 0, 0);
+            }
+          }
+      } else {
+        typedef typename Mma<T>::frag frag;
+        typedef __attribute__((address_space(3))) shortx4 lds4;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            frag p;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[j] = from_f32<T>(s[kb][8 * h + j]);
+            if constexpr (!kAll) p = __builtin_bit_cast(frag, __builtin_bit_cast(u32x4, p) & (slow ? 0u : ~0u));
+            const int row = 32 * kb + 16 * h + 4 * half + ((lane & 15) >> 2);
+#pragma unroll
+            for (int d = 0; d < NB; ++d) {
+              // dimensions past D (16) read the row's first ones; their output is not used
+              const int dim = (D % 32 == 0 ? 32 * d + 16 * ((lane >> 4) & 1) : 0) + 4 * (lane & 3);
+              union {
+                shortx4 h[2];
+                u32x4 w;
+              } u;
+              u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (lds4*)(vs + row * kRowB + (((dim >> 3) ^ swz(row)) << 4) + (dim & 4) * 2));
+              u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (lds4*)(vs + (row + 8) * kRowB + (((dim >> 3) ^ swz(row + 8)) << 4) + (dim & 4) * 2));
+              if constexpr (!kAll) u.w &= slow ? 0u : ~0u;
+              acc[d] = Mma<T>::mma(__builtin_bit_cast(frag, u.w), p, acc[d]);
+            }
+          }
+      }
+      if (!kAll && slow) {
+        // one key at a time, into the rows that see it
+#pragma unroll 1
+        for (int only = 0; only < KT; ++only) {
+          const int half_ = fresh(half);
+          float p = 0.f;   // in the half of the wave that holds the key
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p = 32 * kb + (i & 3) + 8 * (i >> 2) == only - 4 * half_ ? s[kb][i] : p;
+          p = to_f32(from_f32<T>(half_sum(p)));
+          const bool take = key0 + only < lim && !hidden(key0 + only);
+#pragma unroll
+          for (int d = 0; d < NB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int at = min(32 * d + (i & 3) + 8 * (i >> 2) + 4 * half_, D - 1) * (int)sizeof(T);
+              const T v = *reinterpret_cast<const T*>(vs + only * kRowB + (((at >> 4) ^ swz(only)) << 4) + (at & 15));
+              acc[d][i] = take ? __builtin_fmaf(p, to_f32(v), acc[d][i]) : acc[d][i];
+            }
+        }
+      }
+      if constexpr (WR == 1) {
+        if (more) {
+          lds_wait();
+          issue(tile + BN, 0, true);
+        }
+      }
+    };
+    int tile = seg, n = 0;
+    const int whole = bad_pages ? seg : min(all, send);
+#pragma unroll 1
+    for (; tile + BN <= whole; tile += BN, ++n) do_tile(tile, n, std::true_type{});
+#pragma unroll 1
+    for (; tile < send; tile += BN, ++n) do_tile(tile, n, std::false_type{});
+  }
+
+  // ---- the waves of the same rows join: every wave scales its sums to their
+  // largest max, and takes 1 / WK of the rows
+  l = half_sum(l);
+  if (half == 0) {
+    s_ml[(wave * 32 + col) * 2] = m;
+    s_ml[(wave * 32 + col) * 2 + 1] = l;
+  }
+  __syncthreads();   // also: no tile is read any more
+  float M = m, L = l;
+  if constexpr (WK > 1) {
+    M = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < WK; ++k) M = fmaxf(M, s_ml[((k * WR + wr) * 32 + col) * 2]);
+    L = 0.f;
+#pragma unroll
+    for (int k = 0; k < WK; ++k) {
+      const float mk = s_ml[((k * WR + wr) * 32 + col) * 2], lk = s_ml[((k * WR + wr) * 32 + col) * 2 + 1];
+      L += mk == -INFINITY ? lk : lk * exp2_hw(mk - M);   // (a sum without a max is 0, or NaN)
+    }
+    const float w = m == -INFINITY ? 1.f : exp2_hw(m - M);
+#pragma unroll
+    for (int d = 0; d < NB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[d][i] *= w;
+  }
+  constexpr int kOs = D + 4;
+  float* so = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int d = 0; d < NB; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int dim = 32 * d + 8 * (i >> 2) + 4 * half;
+      if (D % 32 == 0 || dim < D)
+        *reinterpret_cast<floatx4*>(so + (wave * 32 + col) * kOs + dim) =
+            floatx4{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
+    }
+  __syncthreads();
+  const int64_t rows_all = (int64_t)a.N * a.Hq;
+  float* po = a.part_o + it.slot * rows_all * D;
+  constexpr int kVec = D / 4;                    // 16-byte pieces of a row
+  constexpr int kJoin = 32 / WK;                 // rows of a wave
+  for (int i = lane; i < kJoin * kVec; i += 64) {
+    const int c = wk * kJoin + i / kVec, dim = (i % kVec) * 4;
+    floatx4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < WK; ++k) x += *reinterpret_cast<const floatx4*>(so + ((k * WR + wr) * 32 + c) * kOs + dim);
+    const int row = it.row0 + 32 * wr + c;
+    if (row < it.rows) {
+      const int64_t ridx = (int64_t)(it.tok0 + row / a.G) * a.Hq + it.hk * a.G + row % a.G;
+      *reinterpret_cast<floatx4*>(po + ridx * D + dim) = x;
+    }
+  }
+  if (wk == 0 && half == 0 && live) {
+    float* ml = a.part_ml + (it.slot * rows_all + (int64_t)tok * a.Hq + head) * 2;
+    ml[0] = M;
+    ml[1] = L;
+  }
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__((PrefixShape<T, D>::kWaves * 64)) __attribute__((amdgpu_waves_per_eu(1, 2))) void
+prefix_attn_kernel(PrefixArgs a) {
+  using Sh = PrefixShape<T, D>;
+  __shared__ __attribute__((aligned(16))) char smem[Sh::kLds];
+  __shared__ int32_t s_pid[kPageIds];
+  __shared__ float s_ml[Sh::kWaves * 64];
+  Item it{};
+  const int tokens = a.cu ? min(max(a.cu[a.B], 0), a.N) : a.N;
+  int x = blockIdx.x;
+  if (x < a.p_items) {
+    const int per = a.Hk * a.p_splits, pair = x % per;
+    it.hk = pair % a.Hk;
+    const int split = pair / a.Hk;
+    it.row0 = x / per * 32 * a.p_wr;
+    it.rows = tokens * a.G;
+    it.kbeg = split * a.p_chunk;
+    it.kend = min(a.S, it.kbeg + a.p_chunk);
+    it.slot = a.o_splits + split;
+    if (it.row0 >= it.rows) return;
+    switch (a.p_wr) {
+      case 1: prefix_item<T, D, 1, false>(a, it, smem, s_pid, s_ml); break;
+      case 2: prefix_item<T, D, 2, false>(a, it, smem, s_pid, s_ml); break;
+      case 4: prefix_item<T, D, 4, false>(a, it, smem, s_pid, s_ml); break;
+      default:
+        if constexpr (Sh::kWaves == 8) prefix_item<T, D, 8, false>(a, it, smem, s_pid, s_ml);
+        break;
+    }
+  } else {
+    x -= a.p_items;
+    it.hk = x % a.Hk;
+    x /= a.Hk;
+    const int split = x % a.o_splits;
+    x /= a.o_splits;
+    const int tile = x % a.o_tiles, b = x / a.o_tiles;
+    int c0 = b, c1 = b + 1;
+    if (a.cu) {
+      c0 = min(max(a.cu[b], 0), tokens);
+      c1 = min(max(a.cu[b + 1], c0), tokens);
+    }
+    const int n = c1 - c0, len = min(max(a.lens[b], 0), a.T << a.lp);
+    it.tok0 = c0;
+    it.row0 = tile * 32 * a.o_wr;
+    it.rows = min(n, a.max_new) * a.G;
+    if (it.row0 >= it.rows) return;
+    const int chunk = own_chunk(len, a.o_splits);
+    it.lim0 = len - n + 1;
+    it.kbeg = min((int64_t)split * chunk, (int64_t)len);
+    const int last = min(it.row0 + 32 * a.o_wr, it.rows) - 1;   // the tile's row that sees most
+    it.kend = min(min(it.kbeg + chunk, len), max(0, it.lim0 + last / a.G));
+    it.table = a.tables + b * a.t_sb;
+    it.slot = split;
+    if (it.kbeg >= it.kend) return;
+    switch (a.o_wr) {
+      case 1: prefix_item<T, D, 1, true>(a, it, smem, s_pid, s_ml); break;
+      case 2: prefix_item<T, D, 2, true>(a, it, smem, s_pid, s_ml); break;
+      case 4: prefix_item<T, D, 4, true>(a, it, smem, s_pid, s_ml); break;
+      default:
+        if constexpr (Sh::kWaves == 8) prefix_item<T, D, 8, true>(a, it, smem, s_pid, s_ml);
+        break;
+    }
+  }
+}
+
+// Joins the partials of every query row: grid m_tiles tiles of kMergeRows rows
+// of each request, D / 4 threads a row.  A partial exists where the row sees
+// keys of its range, and where it does not the row has nothing there.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
+  constexpr int kVec = D / 4, kRows = 256 / kVec;
+  const int b = blockIdx.x / a.m_tiles, tile = blockIdx.x % a.m_tiles;
+  int c0 = b, c1 = b + 1;
+  if (a.cu) {
+    const int tokens = min(max(a.cu[a.B], 0), a.N);
+    c0 = min(max(a.cu[b], 0), tokens);
+    c1 = min(max(a.cu[b + 1], c0), tokens);
+  }
+  const int n = c1 - c0, len = min(max(a.lens[b], 0), a.T << a.lp);
+  const int i = tile * kRows + threadIdx.x / kVec, dim = threadIdx.x % kVec * 4;
+  const int t = i / a.Hq, h = i - t * a.Hq;
+  if (t >= min(n, a.max_new)) return;
+  const int S = a.prefix_lens ? min(max(a.prefix_lens[b], 0), a.S) : a.S;
+  const int own = max(0, len - n + 1 + t), chunk = own_chunk(len, a.o_splits);
+  const int n_own = (min(own, len) + chunk - 1) / chunk, n_pre = a.p_splits ? (S + a.p_chunk - 1) / a.p_chunk : 0;
+  const int64_t rows_all = (int64_t)a.N * a.Hq, ridx = (int64_t)(c0 + t) * a.Hq + h;
+  const int count = n_own + n_pre;
+  auto slot = [&](int s) { return s < n_own ? s : a.o_splits + s - n_own; };
+  float M = -INFINITY;
+  for (int s = 0; s < count; ++s) M = fmaxf(M, a.part_ml[(slot(s) * rows_all + ridx) * 2]);
+  float L = 0.f;
+  floatx4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < count; ++s) {
+    const int64_t at = slot(s) * rows_all + ridx;
+    const float m = a.part_ml[at * 2], l = a.part_ml[at * 2 + 1];
+    const floatx4 o = *reinterpret_cast<const floatx4*>(a.part_o + at * D + dim);
+    const float w = m == -INFINITY ? 1.f : exp2_hw(m - M);   // (sums without a max are 0, or NaN)
+    L += l * w;
+    x += o * w;
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  T* out = reinterpret_cast<T*>(a.out + (c0 + t) * a.o_sn + h * a.o_sh) + dim;
+  typedef T outx4 __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<outx4*>(out) =
+      outx4{from_f32<T>(x[0] * inv), from_f32<T>(x[1] * inv), from_f32<T>(x[2] * inv), from_f32<T>(x[3] * inv)};
+  if (a.lse && dim == 0)
+    a.lse[(c0 + t) * a.l_sn + h * a.l_sh] = L == 0.f ? -INFINITY : (M + __log2f(L)) * 0.6931471805599453f;
+}
+
+template <typename T, int D>
+void launch_prefix_d(const PrefixArgs& a, int64_t items, hipStream_t s) {
+  prefix_attn_kernel<T, D><<<(unsigned)items, PrefixShape<T, D>::kWaves * 64, 0, s>>>(a);
+  prefix_merge_kernel<T, D><<<(unsigned)(a.B * a.m_tiles), 256, 0, s>>>(a);
+}
+
+template <typename T>
+void launch_prefix(const PrefixArgs& a, int64_t items, hipStream_t s) {
+  switch (a.D) {
+    case 16: launch_prefix_d<T, 16>(a, items, s); break;
+    case 32: launch_prefix_d<T, 32>(a, items, s); break;
+    case 64: launch_prefix_d<T, 64>(a, items, s); break;
+    default: launch_prefix_d<T, 128>(a, items, s); break;
+  }
+}
+
+}  // namespace hc
