@@ -16,7 +16,7 @@ constexpr int kCus = 256;
 
 // How a call is laid out over workgroups.
 struct PrefixPlan {
-  int p_wr, p_tiles, p_splits, p_chunk, o_wr, o_tiles, o_splits, m_tiles;
+  int p_wr, p_tiles, p_splits, p_chunk, o_wr, o_tiles, o_splits, m_tiles, both;
   int64_t items, slots;
 };
 
@@ -27,30 +27,53 @@ int rows_waves(int64_t rows, int waves) {
   return wr;
 }
 
+// Times of a workgroup, in ns, as measured at head dimension 128 and 2-byte
+// types: kWgNs of its own (arguments, first loads, the waves' join), and a key's.
+// One CU streams about 40 GB/s, all together kHbm; products of 32 WR rows take
+// the rest (30 ns a key of 256 rows).
+constexpr double kWgNs = 7000, kCuGBs = 40, kHbmGBs = 5000;
+
 PrefixPlan plan_prefix(const hc_prefix_attn_args* x) {
   PrefixPlan p{};
-  const int waves = x->D * dtype_size((int)x->dtype) >= 512 ? 4 : 8;
-  const int64_t G = x->Hq / x->Hk, rows = x->N * G, most = std::min(x->max_new, x->N);
+  const int64_t es = dtype_size((int)x->dtype), G = x->Hq / x->Hk, rows = x->N * G, most = std::min(x->max_new, x->N);
+  const int waves = x->D * es >= 512 ? 4 : 8;
+  const double key_bytes = 2.0 * (double)(x->D * es);
+  auto key_ns = [&](int wr) { return std::max(key_bytes / kCuGBs, 3.75 * wr * 8 / waves * (double)(x->D * es * es) / 512); };
+  p.o_wr = rows_waves(most * G, waves);
+  p.o_tiles = (int)cdiv(most * G, 32 * p.o_wr);
+  // Own items: a request's keys are split only as far as it takes to give every
+  // CU some.  Their lengths are on the device; half of what the table holds is
+  // taken for the mean.
+  const int64_t units = x->B * x->Hk * p.o_tiles, longest = x->table_width * x->page_size;
+  p.o_splits = (int)std::max<int64_t>(1, std::min<int64_t>({cdiv((int64_t)kCus / 2, units), cdiv(longest, (int64_t)256), 64}));
+  const double own_keys = 0.5 * (double)longest / p.o_splits;
+  const double own_n = (double)units * p.o_splits, own_ns = kWgNs + own_keys * key_ns(p.o_wr);
   if (x->prefix_rows > 0) {
     p.p_wr = rows_waves(rows, waves);
     p.p_tiles = (int)cdiv(rows, 32 * p.p_wr);
-    const int64_t bn = p.p_wr == waves ? 64 : 32 * (waves / p.p_wr), units = p.p_tiles * x->Hk;
-    // the fewest rounds of workgroups times a workgroup's keys and fixed cost
-    int64_t best = INT64_MAX;
-    for (int64_t s = 1; s <= 256 && s <= cdiv(x->prefix_rows, bn); ++s) {
+    const int64_t bn = p.p_wr == waves ? 64 : std::max(128, 32 * (waves / p.p_wr)), units_p = p.p_tiles * x->Hk;
+    // Prompt items go first, and the own ones on the CUs they leave.  With s
+    // splits they take t; by then each CU left has done t / own_ns own items,
+    // and what remains of them runs on all CUs (or at the memory's rate).
+    double best = 0;
+    for (int64_t s = 1; s <= 512; s += 1 + s / 12) {
       const int64_t chunk = cdiv(cdiv(x->prefix_rows, s), bn) * bn, splits = cdiv(x->prefix_rows, chunk);
-      const int64_t cost = cdiv(units * splits, (int64_t)kCus) * (chunk + 256);
-      if (cost < best) {
-        best = cost;
+      const double n = (double)(units_p * splits), rounds = std::ceil(n / kCus);
+      const double left = std::max(0.0, kCus - n);
+      double t = rounds * (kWgNs + (double)chunk * key_ns(p.p_wr));
+      const double done = std::min(own_n, left * std::floor(t / own_ns));
+      t = std::max(t, (n * (double)chunk + done * own_keys) * key_bytes / kHbmGBs);
+      const double rest = own_n - done;
+      if (rest > 0) t += std::max(std::ceil(rest / kCus) * own_ns, rest * own_keys * key_bytes / kHbmGBs);
+      t += (double)(splits * rows * x->Hk * x->D * 8) / kHbmGBs;   // partials, written and read
+      if (p.p_splits == 0 || t < best) {
+        best = t;
         p.p_splits = (int)splits;
         p.p_chunk = (int)chunk;
       }
+      if (chunk == bn) break;
     }
   }
-  p.o_wr = rows_waves(most * G, waves);
-  p.o_tiles = (int)cdiv(most * G, 32 * p.o_wr);
-  const int64_t units = x->B * x->Hk * p.o_tiles, longest = x->table_width * x->page_size;
-  p.o_splits = (int)std::max<int64_t>(1, std::min<int64_t>({cdiv((int64_t)(4 * kCus), units), cdiv(longest, (int64_t)256), 64}));
   p.m_tiles = (int)cdiv(most * x->Hq * (x->D / 4), (int64_t)256);
   p.items = (int64_t)p.p_tiles * x->Hk * p.p_splits + units * p.o_splits;
   p.slots = p.p_splits + p.o_splits;
@@ -147,7 +170,7 @@ extern "C" int hc_prefix_attn(const hc_prefix_attn_args* x, void* stream) {
   a.max_new = (int)std::min<int64_t>(x->max_new, x->N);
   a.p_wr = p.p_wr; a.p_tiles = p.p_tiles; a.p_splits = p.p_splits; a.p_chunk = p.p_chunk;
   a.p_items = p.p_tiles * a.Hk * p.p_splits;
-  a.o_wr = p.o_wr; a.o_tiles = p.o_tiles; a.o_splits = p.o_splits; a.m_tiles = p.m_tiles;
+  a.o_wr = p.o_wr; a.o_tiles = p.o_tiles; a.o_splits = p.o_splits; a.both = p.both; a.m_tiles = p.m_tiles;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (dtype == HC_DTYPE_F16) launch_prefix<half_t>(a, p.items, s);
   else if (dtype == HC_DTYPE_BF16) launch_prefix<bf16_t>(a, p.items, s);

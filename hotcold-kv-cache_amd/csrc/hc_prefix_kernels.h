@@ -79,6 +79,7 @@ struct PrefixArgs {
   // split; own items: WR, row tiles and splits of one request
   int p_wr, p_tiles, p_splits, p_chunk, p_items;
   int o_wr, o_tiles, o_splits;
+  int both;   // own items take the prompt too: no prompt items, no partials
   // merge: tiles of rows of one request
   int m_tiles;
 };
@@ -86,13 +87,17 @@ struct PrefixArgs {
 constexpr float kLazy = 8.f;
 constexpr int kPageIds = 2048;  // page numbers held in LDS at a time
 
+// NW waves a workgroup, one workgroup a CU (256 registers a lane, most of LDS):
+// 8, or 4 where rows are 512 bytes, as K and V of 32 keys a wave have to fit
+// LDS.  (Workgroups of 4 waves, two a CU, took longer at every split: 16
+// requests behind 32k prompt rows 51 us against 68, 64 behind 64k 139 / 180.)
 template <typename T, int D>
 struct PrefixShape {
   static constexpr int kRowB = D * (int)sizeof(T);
-  static constexpr int kWaves = kRowB >= 512 ? 4 : 8;  // K and V of 32 keys a wave fit LDS
+  static constexpr int NW = kRowB >= 512 ? 4 : 8;
   static constexpr int kPieces = kRowB / 16;
-  static constexpr int kTileB = kWaves * 32 * 2 * kRowB;   // WR = 1: one buffer; WR >= 2: two of BN keys
-  static constexpr int kOutB = kWaves * 32 * (D + 4) * 4;  // the outputs of all waves
+  static constexpr int kTileB = NW * 32 * 2 * kRowB;   // WR = 1: one buffer; more: two of BN keys
+  static constexpr int kOutB = NW * 32 * (D + 4) * 4;  // the outputs of all waves
   static constexpr int kLds = kTileB > kOutB ? kTileB : kOutB;
 };
 
@@ -118,17 +123,17 @@ __device__ __forceinline__ float half_sum(float x) {
 // wave's) + 16 * lane, asynchronously: complete after vm_wait.  The compiler
 // does not see the write; every use is behind a vm_wait, which it does not
 // move memory accesses across.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ void load_to_lds(const void* p, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(uniform(lds)), "v"(p)
+               : "memory");
 }
 // ... from the wave's address base plus the lane's offset.  (The base may come
 // from a v_readfirstlane, which takes five wait states before a memory
 // instruction may read it; the compiler's own count does not look into asm.)
 __device__ __forceinline__ void load_to_lds(const void* base, uint32_t off, uint32_t lds) {
-  const uint64_t at = (uint64_t)base;
-  const uint64_t s = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32 |
-                     (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(s)
+  const uint64_t s = (uint64_t)uniform((uint32_t)((uint64_t)base >> 32)) << 32 | uniform((uint32_t)(uint64_t)base);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(uniform(lds)), "v"(off), "s"(s)
                : "memory");
 }
 __device__ __forceinline__ void lds_wait() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
@@ -162,23 +167,43 @@ struct Mma<bf16_t> {
 };
 template <>
 struct Mma<float> {
-  typedef floatx4 frag;
+  typedef floatx4 frag;   // four products of two dimensions each
+  __device__ static floatx16 mma(floatx4 a, floatx4 b, floatx16 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
 };
 
-// What an item's workgroup works on.
+// What an item's workgroup works on: the prompt's keys, a request's own, or
+// both, one after the other (then the rows are complete and go out as they are).
+enum { kPromptItem, kOwnItem, kBothItem };
 struct Item {
   int hk, tok0, row0, rows;   // query rows [row0, rows) of tokens tok0 + row / G
-  int kbeg, kend;             // keys
-  int lim0, cut;              // own items: row r sees keys below lim0 + r / G (at least 0)
-  const int32_t* table;       // own items: the request's pages
-  int slot;                   // where its partial goes
+  int pbeg, pend;             // the prompt's keys
+  int obeg, oend;             // own keys; row r sees those below lim0 + r / G (at least 0)
+  int lim0;
+  const int32_t* table;       // the request's pages
+  int slot;                   // where the partial goes
 };
 
-template <typename T, int D, int WR, bool kOwn>
+// Four dimensions of a complete row, and its log-sum-exp.
+template <typename T>
+__device__ __forceinline__ void finish_row(const PrefixArgs& a, int t, int h, int dim, floatx4 x, float M, float L) {
+  typedef T outx4 __attribute__((ext_vector_type(4)));
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  *reinterpret_cast<outx4*>(reinterpret_cast<T*>(a.out + t * a.o_sn + h * a.o_sh) + dim) =
+      outx4{from_f32<T>(x[0] * inv), from_f32<T>(x[1] * inv), from_f32<T>(x[2] * inv), from_f32<T>(x[3] * inv)};
+  if (a.lse && dim == 0)
+    a.lse[t * a.l_sn + h * a.l_sh] = L == 0.f ? -INFINITY : (M + __log2f(L)) * 0.6931471805599453f;
+}
+
+template <typename T, int D, int WR, int kMode>
 __device__ __forceinline__ void prefix_item(const PrefixArgs& a, const Item& it, char* smem, int32_t* s_pid, float* s_ml) {
   using Sh = PrefixShape<T, D>;
-  constexpr int kRowB = Sh::kRowB, kPieces = Sh::kPieces, WK = Sh::kWaves / WR;
-  constexpr int KT = WK == 1 ? 64 : 32;        // keys a wave takes of a tile
+  constexpr int NW = Sh::NW;
+  constexpr int kRowB = Sh::kRowB, kPieces = Sh::kPieces, WK = NW / WR;
+  constexpr int KT = WK <= NW / 4 ? 64 : 32;   // keys a wave takes of a tile
   constexpr int KB = KT / 32, BN = WK * KT;
   constexpr int kStages = WR == 1 ? 1 : 2;
   constexpr int kRows = KT / WR;               // rows of a tile a wave loads
@@ -189,6 +214,7 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, const Item& it,
   static_assert(2 * kSt * kStages <= Sh::kLds, "tiles fit LDS");
   constexpr int NB = (D + 31) / 32;            // blocks of 32 output dimensions
   constexpr bool kF32 = sizeof(T) == 4;
+  typedef typename Mma<T>::frag frag;
   constexpr int NQ = kF32 ? D / 8 : (D + 15) / 16;
 
   const int lane = threadIdx.x & 63;
@@ -213,65 +239,12 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, const Item& it,
       qf[t] = __builtin_bit_cast(typename Mma<T>::frag, x);
     }
   }
-  int lim = it.kend;
-  if constexpr (kOwn) {
-    if (live) lim = min(lim, max(0, it.lim0 + r / a.G));
-  } else {
-    if (live && a.prefix_lens) {
-      int b = tok;
-      if (a.cu) {   // the last request that starts at or before the token
-        int lo = 0, hi = a.B - 1;
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if (a.cu[mid] <= tok) lo = mid; else hi = mid - 1;
-        }
-        b = lo;
-      }
-      lim = min(lim, max(0, a.prefix_lens[b]));
-    }
-  }
-  // keys every row of the workgroup sees, and keys some row sees
-  int all = it.kend, kend = it.kend;
-  if constexpr (kOwn) {
-    all = min(it.kend, max(0, it.lim0 + it.row0 / a.G));   // (the first row sees least; kend is the last's)
-  } else if (a.prefix_lens) {
-    int lo = lim, hi = live ? lim : 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      lo = min(lo, __shfl_xor(lo, o, 64));
-      hi = max(hi, __shfl_xor(hi, o, 64));
-    }
-    int* s_lim = reinterpret_cast<int*>(s_ml);
-    if (lane == 0) {
-      s_lim[wave] = lo;
-      s_lim[Sh::kWaves + wave] = hi;
-    }
-    __syncthreads();
-    kend = 0;
-#pragma unroll
-    for (int w = 0; w < Sh::kWaves; ++w) {
-      all = min(all, s_lim[w]);
-      kend = max(kend, s_lim[Sh::kWaves + w]);
-    }
-    all = __builtin_amdgcn_readfirstlane(all);
-    kend = __builtin_amdgcn_readfirstlane(kend);
-    __syncthreads();
-  }
-  // rows see different keys: a value that is not finite may have to reach some
-  // of them only
-  const bool ragged = all != kend;
-
   floatx16 acc[NB];
 #pragma unroll
   for (int d = 0; d < NB; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
   float m = -INFINITY, l = 0.f;
-
-  const char* kbase = kOwn ? a.kg + it.hk * a.kg_sh : a.kp + it.hk * a.kp_sh;
-  const char* vbase = kOwn ? a.vg + it.hk * a.vg_sh : a.vp + it.hk * a.vp_sh;
-  // (a segment's first page may be entered in its middle)
-  const int seg_keys = kOwn ? ((kPageIds - 1) << min(a.lp, 12)) / BN * BN : 0x7fffffff;
 
   // f(r) of row r: pieces of 16 rows with the same number lie on distinct
   // 16-byte columns of the 256 bytes all banks hold, pairs of 4 rows too
@@ -283,48 +256,67 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, const Item& it,
     return ((x << 1) | (x >> (kXorBits - 1))) & (kXor - 1);
   };
 
-  for (int seg = it.kbeg, send; seg < kend; seg = send) {
+  // The keys [kbeg, kend) of the prompt or of the request's pages: the lane's
+  // row sees those below lim, every row of the workgroup those below all.
+  auto sweep = [&](auto own_keys, const int kbeg, const int kend, const int all, const int lim) {
+  constexpr bool kOwn = decltype(own_keys)::value;
+  // rows see different keys: a value that is not finite may have to reach some
+  // of them only
+  const bool ragged = all != kend;
+  const char* kbase = kOwn ? a.kg + it.hk * a.kg_sh : a.kp + it.hk * a.kp_sh;
+  const char* vbase = kOwn ? a.vg + it.hk * a.vg_sh : a.vp + it.hk * a.vp_sh;
+  // (a segment's first page may be entered in its middle)
+  const int seg_keys = kOwn ? ((kPageIds - 1) << min(a.lp, 12)) / BN * BN : 0x7fffffff;
+  for (int seg = kbeg, send; seg < kend; seg = send) {
     send = kend - seg > seg_keys ? seg + seg_keys : kend;
     bool bad_pages = false;
     const int page0 = seg >> a.lp;
     if constexpr (kOwn) {
-      // (the barrier also keeps the last segment's tiles until all are read)
-      __syncthreads();
+      if (seg != kbeg) __syncthreads();   // the last segment's pages are read
       int bad = 0;
       const int n = ((send - 1) >> a.lp) - page0 + 1;
-      for (int i = threadIdx.x; i < n; i += Sh::kWaves * 64) {
+      for (int i = threadIdx.x; i < n; i += NW * 64) {
         const int p = it.table[page0 + i];
         const bool ok = (uint32_t)p < (uint32_t)a.num_pages;
         s_pid[i] = ok ? p : -1;
         bad |= !ok;
       }
-      bad_pages = __builtin_amdgcn_readfirstlane(__syncthreads_or(bad)) != 0;
+      int* s_bad = reinterpret_cast<int*>(s_ml);
+      bad = __any(bad);
+      if (lane == 0) s_bad[wave] = bad;
+      __syncthreads();   // (also: the tiles of the keys before are read)
+      int any = 0;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) any |= s_bad[w];
+      bad_pages = __builtin_amdgcn_readfirstlane(any) != 0;
     }
 
-    // asynchronous loads of the wave's rows of the tile at key0; a load's rows
-    // are consecutive keys: of one page where pages hold that many
+    // asynchronous loads of the wave's rows of the tile at key0: consecutive
+    // keys, one address and the lanes' offsets where they are in one page
     auto issue = [&](int key0, int stage, bool v) {
       const int piece = lane % kPieces, sub = lane / kPieces;
       const uint32_t dst = lds0 + (uint32_t)((stage * 2 + (v ? 1 : 0)) * kSt + (wk * KT + wr * kRows) * kRowB);
       const int64_t ss = kOwn ? (v ? a.vg_ss : a.kg_ss) : (v ? a.vp_ss : a.kp_ss);
       const char* base = v ? vbase : kbase;
       const int first = key0 + wk * KT + wr * kRows;
-      const bool whole = first + kRows <= send && (!kOwn || (1 << a.lp) >= kPerLoad);
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j) {
-        const uint32_t d = __builtin_amdgcn_readfirstlane(dst + (uint32_t)(j * 1024));
-        const int at = 16 * (piece ^ swz(wr * kRows + j * kPerLoad + sub));
-        if (whole) {
-          const int key = first + j * kPerLoad;
-          const char* p = base;
-          if constexpr (kOwn) {
-            const int pid = __builtin_amdgcn_readfirstlane(s_pid[(key >> a.lp) - page0]);
-            p += (int64_t)max(pid, 0) * (v ? a.vg_sp : a.kg_sp) + (int64_t)(key & ((1 << a.lp) - 1)) * ss;
-          } else {
-            p += (int64_t)key * ss;
-          }
-          if (!kPartial || lane < kRows * kPieces) load_to_lds(p, (uint32_t)sub * (uint32_t)ss + (uint32_t)at, d);
+      // (f of a sum of rows with distinct bits is the xor of theirs)
+      const uint32_t at = 16 * (piece ^ swz(wr * kRows + sub));
+      if (first + kRows <= send && (!kOwn || (1 << a.lp) >= kRows)) {
+        if constexpr (kOwn) {
+          const int pid = __builtin_amdgcn_readfirstlane(s_pid[(first >> a.lp) - page0]);
+          base += (int64_t)max(pid, 0) * (v ? a.vg_sp : a.kg_sp) + (int64_t)(first & ((1 << a.lp) - 1)) * ss;
         } else {
+          base += (int64_t)first * ss;
+        }
+        const uint32_t rows = (uint32_t)sub * (uint32_t)ss;
+        if (!kPartial || lane < kRows * kPieces) {
+#pragma unroll
+          for (int j = 0; j < kLoads; ++j)
+            load_to_lds(base + j * kPerLoad * ss, (at ^ (16 * swz(j * kPerLoad))) + rows, dst + j * 1024);
+        }
+      } else {
+#pragma unroll 1
+        for (int j = 0; j < kLoads; ++j) {
           // keys past the end load the last one's row (zeroed below)
           const int key = min(first + j * kPerLoad + sub, send - 1);
           const char* p = base;
@@ -334,7 +326,7 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, const Item& it,
           } else {
             p += (int64_t)key * ss;
           }
-          if (!kPartial || lane < kRows * kPieces) load_to_lds(p + at, d);
+          if (!kPartial || lane < kRows * kPieces) load_to_lds(p + (at ^ (16 * swz(j * kPerLoad))), dst + j * 1024);
         }
       }
     };
@@ -355,10 +347,109 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, const Item& it,
       }
     };
 
-    issue(seg, 0, false);
-    issue(seg, 0, true);
+    // scores of the wave's keys of a tile
+    auto qk = [&](const char* ks, floatx16 (&s)[KB]) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
+#pragma unroll
+      for (int t = 0; t < NQ; ++t)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          const int row = 32 * kb + col;
+          const u32x4 x = ld16(ks + row * kRowB + (((2 * t + half) ^ swz(row)) << 4));
+          s[kb] = Mma<T>::mma(__builtin_bit_cast(frag, x), qf[t], s[kb]);
+        }
+    };
+    // scores to probabilities (against the row's reference), and their sum
+    auto softmax = [&](floatx16 (&s)[KB]) {
+      float t = s[0][0], u = s[0][1];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          t = fmaxf(fmaxf(t, s[kb][i]), s[kb][i + 1]);
+          u = fmaxf(fmaxf(u, s[kb][i + 2]), s[kb][i + 3]);
+        }
+      t = half_max(fmaxf(t, u)) * a.scale_log2;
+      const bool bump = t > m + kLazy;
+      if (__any(bump)) {
+        const float mn = bump ? t : m;
+        const float alpha = bump ? exp2_hw(m - mn) : 1.f;
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < NB; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
+      }
+      const float ref = m == -INFINITY ? 0.f : m;   // (a row that has seen nothing yet: its terms are 0)
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          s[kb][i] = exp2_hw(__builtin_fmaf(s[kb][i], a.scale_log2, -ref));
+          sum[i & 3] += s[kb][i];
+        }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    };
+    // probabilities of 16 keys as a product's operand
+    auto pack = [&](const floatx16 (&s)[KB], frag (&p)[2 * KB]) {
+#pragma unroll
+      for (int h = 0; h < 2 * KB; ++h)
+#pragma unroll
+        for (int j = 0; j < 16 / (int)sizeof(T); ++j) p[h][j] = from_f32<T>(s[h / 2][8 * (h & 1) + j]);
+    };
+    // output of the wave's keys of a tile (2-byte types); with zero, of zeros
+    auto pv = [&](const char* vs, const frag (&p)[2 * KB], auto may_zero, bool zero) {
+      typedef __attribute__((address_space(3))) shortx4 lds4;
+#pragma unroll
+      for (int h = 0; h < 2 * KB; ++h) {
+        const int row = 16 * h + 4 * half + ((lane & 15) >> 2);
+#pragma unroll
+        for (int d = 0; d < NB; ++d) {
+          // dimensions past D (16) read the row's first ones; their output is not used
+          const int dim = (D % 32 == 0 ? 32 * d + 16 * ((lane >> 4) & 1) : 0) + 4 * (lane & 3);
+          union {
+            shortx4 h[2];
+            u32x4 w;
+          } u;
+          u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds4*)(vs + row * kRowB + (((dim >> 3) ^ swz(row)) << 4) + (dim & 4) * 2));
+          u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds4*)(vs + (row + 8) * kRowB + (((dim >> 3) ^ swz(row + 8)) << 4) + (dim & 4) * 2));
+          frag f = p[h];
+          if constexpr (decltype(may_zero)::value) {
+            const uint32_t mask = zero ? 0u : ~0u;
+            u.w &= mask;
+            f = __builtin_bit_cast(frag, __builtin_bit_cast(u32x4, f) & mask);
+          }
+          acc[d] = Mma<T>::mma(__builtin_bit_cast(frag, u.w), f, acc[d]);
+        }
+      }
+    };
+    // the order of a phase's LDS reads and products: operands a few products ahead
+    auto order = [](auto products, auto reads, auto ahead, auto id) {
+      constexpr int kN = decltype(products)::value, kR = decltype(reads)::value, kId = decltype(id)::value;
+      constexpr int kA = kN < decltype(ahead)::value ? kN : decltype(ahead)::value;
+      __builtin_amdgcn_sched_group_barrier(0x100, kR * kA, kId);
+      static_for<kN - kA>([](auto) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, kId);
+        __builtin_amdgcn_sched_group_barrier(0x100, kR, kId);
+      });
+      __builtin_amdgcn_sched_group_barrier(0x8, kA, kId);
+    };
+    using std::integral_constant;
+    typedef integral_constant<int, NQ * KB> QkProducts;
+    typedef integral_constant<int, 2 * KB * NB> PvProducts;
+    auto tile_k = [&](int stage) { return smem + stage * 2 * kSt + wk * KT * kRowB; };
+
+    int tile = seg;
+    const int whole = bad_pages ? seg : min(all, send);
     // one tile; kAll: every row sees all of its keys
-    auto do_tile = [&](int tile, int n, auto all_see) {
+    auto do_tile = [&](int n, auto all_see) {
       constexpr bool kAll = decltype(all_see)::value;
       const int stage = kStages == 1 ? 0 : (n & 1);
       const bool more = tile + BN < send;
@@ -379,40 +470,21 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, const Item& it,
           issue(tile + BN, stage ^ 1, true);
         }
       }
-      const char* ks = smem + stage * 2 * kSt + wk * KT * kRowB;
+      const char* ks = tile_k(stage);
       const char* vs = ks + kSt;
       const int key0 = tile + wk * KT;
 
-      // ---- scores
       floatx16 s[KB];
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
-#pragma unroll
-      for (int t = 0; t < NQ; ++t)
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          const int row = 32 * kb + col;
-          const u32x4 x = ld16(ks + row * kRowB + (((2 * t + half) ^ swz(row)) << 4));
-          if constexpr (kF32) {
-            const floatx4 f = __builtin_bit_cast(floatx4, x);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(f[j], qf[t][j], s[kb], 0, 0, 0);
-          } else {
-            s[kb] = Mma<T>::mma(__builtin_bit_cast(typename Mma<T>::frag, x), qf[t], s[kb]);
-          }
-        }
+      qk(ks, s);
+      if constexpr (kAll && !kF32)
+        order(QkProducts{}, integral_constant<int, 1>{}, integral_constant<int, 6>{}, integral_constant<int, 0>{});
       if constexpr (WR == 1) {
         if (more) {
           lds_wait();   // the tile's reads are done
           issue(tile + BN, 0, false);
         }
       }
-
       __builtin_amdgcn_sched_barrier(0);
-      // ---- softmax
       if constexpr (!kAll) {
         const int first = key0 + 4 * fresh(half);
 #pragma unroll
@@ -425,40 +497,12 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, const Item& it,
             s[kb][i] = see ? s[kb][i] : -INFINITY;
           }
       }
-      float t = s[0][0];
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) t = fmaxf(t, s[kb][i]);
-      t = half_max(t) * a.scale_log2;
-      const bool bump = t > m + kLazy;
-      if (__any(bump)) {
-        const float mn = bump ? t : m;
-        const float alpha = bump ? exp2_hw(m - mn) : 1.f;
-        m = mn;
-        l *= alpha;
-#pragma unroll
-        for (int d = 0; d < NB; ++d)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
-      }
-      const float ref = m == -INFINITY ? 0.f : m;   // (a row that has seen nothing yet: its terms are 0)
-      float sum = 0.f;
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[kb][i] = exp2_hw(__builtin_fmaf(s[kb][i], a.scale_log2, -ref));
-          sum += s[kb][i];
-        }
-      l += sum;
+      softmax(s);
       if constexpr (WR == 1) {
         if (more) vm_wait<kLoads>(); else vm_wait<0>();
         if (edge) clear(tile, 0, true);
       }
-
       __builtin_amdgcn_sched_barrier(0);
-      // ---- output
       bool slow = false;
       if (!kAll && ragged) {
         // a value that is not finite in this tile?
@@ -478,7 +522,6 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, const Item& it,
         }
         slow = __any(odd);
       }
-      // (with slow the product is taken of zeros)
       if constexpr (kF32) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
@@ -498,33 +541,11 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, const Item& it,
             }
           }
       } else {
-        typedef typename Mma<T>::frag frag;
-        typedef __attribute__((address_space(3))) shortx4 lds4;
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            frag p;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) p[j] = from_f32<T>(s[kb][8 * h + j]);
-            if constexpr (!kAll) p = __builtin_bit_cast(frag, __builtin_bit_cast(u32x4, p) & (slow ? 0u : ~0u));
-            const int row = 32 * kb + 16 * h + 4 * half + ((lane & 15) >> 2);
-#pragma unroll
-            for (int d = 0; d < NB; ++d) {
-              // dimensions past D (16) read the row's first ones; their output is not used
-              const int dim = (D % 32 == 0 ? 32 * d + 16 * ((lane >> 4) & 1) : 0) + 4 * (lane & 3);
-              union {
-                shortx4 h[2];
-                u32x4 w;
-              } u;
-              u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                  (lds4*)(vs + row * kRowB + (((dim >> 3) ^ swz(row)) << 4) + (dim & 4) * 2));
-              u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                  (lds4*)(vs + (row + 8) * kRowB + (((dim >> 3) ^ swz(row + 8)) << 4) + (dim & 4) * 2));
-              if constexpr (!kAll) u.w &= slow ? 0u : ~0u;
-              acc[d] = Mma<T>::mma(__builtin_bit_cast(frag, u.w), p, acc[d]);
-            }
-          }
+        frag p[2 * KB];
+        pack(s, p);
+        pv(vs, p, integral_constant<bool, !kAll>{}, slow);
+        if constexpr (kAll)
+          order(PvProducts{}, integral_constant<int, 2>{}, integral_constant<int, 4>{}, integral_constant<int, 1>{});
       }
       if (!kAll && slow) {
         // one key at a time, into the rows that see it
@@ -555,80 +576,124 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, const Item& it,
         }
       }
     };
-    int tile = seg, n = 0;
-    const int whole = bad_pages ? seg : min(all, send);
+    if (tile < send) {
+      int n = 0;
+      issue(tile, 0, false);
+      issue(tile, 0, true);
 #pragma unroll 1
-    for (; tile + BN <= whole; tile += BN, ++n) do_tile(tile, n, std::true_type{});
+      for (; tile + BN <= whole; tile += BN, ++n) do_tile(n, std::true_type{});
 #pragma unroll 1
-    for (; tile < send; tile += BN, ++n) do_tile(tile, n, std::false_type{});
+      for (; tile < send; tile += BN, ++n) do_tile(n, std::false_type{});
+    }
   }
 
-  // ---- the waves of the same rows join: every wave scales its sums to their
-  // largest max, and takes 1 / WK of the rows
-  l = half_sum(l);
-  if (half == 0) {
-    s_ml[(wave * 32 + col) * 2] = m;
-    s_ml[(wave * 32 + col) * 2 + 1] = l;
-  }
-  __syncthreads();   // also: no tile is read any more
-  float M = m, L = l;
-  if constexpr (WK > 1) {
-    M = -INFINITY;
+  };
+  if constexpr (kMode == kPromptItem) {
+    int lim = it.pend, all = it.pend, kend = it.pend;
+    if (a.prefix_lens) {
+      if (live) {
+        int b = tok;
+        if (a.cu) {   // the last request that starts at or before the token
+          int lo = 0, hi = a.B - 1;
+          while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (a.cu[mid] <= tok) lo = mid; else hi = mid - 1;
+          }
+          b = lo;
+        }
+        lim = min(lim, max(0, a.prefix_lens[b]));
+      }
+      // keys every row of the workgroup sees, and keys some row sees
+      int lo = lim, hi = live ? lim : 0;
 #pragma unroll
-    for (int k = 0; k < WK; ++k) M = fmaxf(M, s_ml[((k * WR + wr) * 32 + col) * 2]);
-    L = 0.f;
+      for (int o = 16; o > 0; o >>= 1) {
+        lo = min(lo, __shfl_xor(lo, o, 64));
+        hi = max(hi, __shfl_xor(hi, o, 64));
+      }
+      int* s_lim = reinterpret_cast<int*>(s_ml);
+      if (lane == 0) {
+        s_lim[wave] = lo;
+        s_lim[NW + wave] = hi;
+      }
+      __syncthreads();
+      kend = 0;
 #pragma unroll
-    for (int k = 0; k < WK; ++k) {
-      const float mk = s_ml[((k * WR + wr) * 32 + col) * 2], lk = s_ml[((k * WR + wr) * 32 + col) * 2 + 1];
-      L += mk == -INFINITY ? lk : lk * exp2_hw(mk - M);   // (a sum without a max is 0, or NaN)
+      for (int w = 0; w < NW; ++w) {
+        all = min(all, s_lim[w]);
+        kend = max(kend, s_lim[NW + w]);
+      }
+      all = __builtin_amdgcn_readfirstlane(all);
+      kend = __builtin_amdgcn_readfirstlane(kend);
     }
-    const float w = m == -INFINITY ? 1.f : exp2_hw(m - M);
+    sweep(std::false_type{}, it.pbeg, kend, all, lim);
+  }
+  if constexpr (kMode == kBothItem) sweep(std::false_type{}, it.pbeg, it.pend, it.pend, it.pend);
+  if constexpr (kMode != kPromptItem) {
+    // (the first row sees least; oend is the last one's)
+    const int all = min(it.oend, max(0, it.lim0 + it.row0 / a.G));
+    sweep(std::true_type{}, it.obeg, it.oend, all, live ? min(it.oend, max(0, it.lim0 + r / a.G)) : it.oend);
+  }
+
+  // ---- the waves of the same rows join: through LDS, each row's sums weighted
+  // by its waves' maxima
+  l = half_sum(l);
+  constexpr int kOs = D + 4;
+  float* so = reinterpret_cast<float*>(smem);
+  __syncthreads();   // no tile is read any more
+  if (live) {
+    if (half == 0) {
+      s_ml[(wave * 32 + col) * 2] = m;
+      s_ml[(wave * 32 + col) * 2 + 1] = l;
+    }
 #pragma unroll
     for (int d = 0; d < NB; ++d)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[d][i] *= w;
+      for (int i = 0; i < 16; i += 4) {
+        const int dim = 32 * d + 8 * (i >> 2) + 4 * half;
+        if (D % 32 == 0 || dim < D)
+          *reinterpret_cast<floatx4*>(so + (wave * 32 + col) * kOs + dim) =
+              floatx4{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
+      }
   }
-  constexpr int kOs = D + 4;
-  float* so = reinterpret_cast<float*>(smem);
-#pragma unroll
-  for (int d = 0; d < NB; ++d)
-#pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const int dim = 32 * d + 8 * (i >> 2) + 4 * half;
-      if (D % 32 == 0 || dim < D)
-        *reinterpret_cast<floatx4*>(so + (wave * 32 + col) * kOs + dim) =
-            floatx4{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
-    }
   __syncthreads();
   const int64_t rows_all = (int64_t)a.N * a.Hq;
-  float* po = a.part_o + it.slot * rows_all * D;
   constexpr int kVec = D / 4;                    // 16-byte pieces of a row
-  constexpr int kJoin = 32 / WK;                 // rows of a wave
-  for (int i = lane; i < kJoin * kVec; i += 64) {
-    const int c = wk * kJoin + i / kVec, dim = (i % kVec) * 4;
+  const int first = it.row0 + 32 * wr, join = min(32, it.rows - first);   // the waves' live rows
+  for (int i = wk * 64 + lane; i < join * kVec; i += 64 * WK) {
+    const int c = i / kVec, dim = (i % kVec) * 4;
+    float M = -INFINITY, L = 0.f;
     floatx4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < WK; ++k) x += *reinterpret_cast<const floatx4*>(so + ((k * WR + wr) * 32 + c) * kOs + dim);
-    const int row = it.row0 + 32 * wr + c;
-    if (row < it.rows) {
-      const int64_t ridx = (int64_t)(it.tok0 + row / a.G) * a.Hq + it.hk * a.G + row % a.G;
-      *reinterpret_cast<floatx4*>(po + ridx * D + dim) = x;
+    for (int k = 0; k < WK; ++k) M = fmaxf(M, s_ml[((k * WR + wr) * 32 + c) * 2]);
+#pragma unroll
+    for (int k = 0; k < WK; ++k) {
+      const int w = (k * WR + wr) * 32 + c;
+      const float mk = s_ml[w * 2], scale = mk == -INFINITY ? 1.f : exp2_hw(mk - M);   // (no max: 0, or NaN)
+      L += s_ml[w * 2 + 1] * scale;
+      x += *reinterpret_cast<const floatx4*>(so + w * kOs + dim) * scale;
     }
-  }
-  if (wk == 0 && half == 0 && live) {
-    float* ml = a.part_ml + (it.slot * rows_all + (int64_t)tok * a.Hq + head) * 2;
-    ml[0] = M;
-    ml[1] = L;
+    const int row = first + c, t = it.tok0 + row / a.G, h = it.hk * a.G + row % a.G;
+    if constexpr (kMode == kBothItem) {
+      finish_row<T>(a, t, h, dim, x, M, L);
+    } else {
+      const int64_t at = it.slot * rows_all + (int64_t)t * a.Hq + h;
+      *reinterpret_cast<floatx4*>(a.part_o + at * D + dim) = x;
+      if (dim == 0) {
+        a.part_ml[at * 2] = M;
+        a.part_ml[at * 2 + 1] = L;
+      }
+    }
   }
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__((PrefixShape<T, D>::kWaves * 64)) __attribute__((amdgpu_waves_per_eu(1, 2))) void
+__global__ __launch_bounds__((PrefixShape<T, D>::NW * 64)) __attribute__((amdgpu_waves_per_eu(1, 2))) void
 prefix_attn_kernel(PrefixArgs a) {
   using Sh = PrefixShape<T, D>;
+  constexpr int NW = Sh::NW;
   __shared__ __attribute__((aligned(16))) char smem[Sh::kLds];
   __shared__ int32_t s_pid[kPageIds];
-  __shared__ float s_ml[Sh::kWaves * 64];
+  __shared__ float s_ml[NW * 64];
   Item it{};
   const int tokens = a.cu ? min(max(a.cu[a.B], 0), a.N) : a.N;
   int x = blockIdx.x;
@@ -638,16 +703,16 @@ prefix_attn_kernel(PrefixArgs a) {
     const int split = pair / a.Hk;
     it.row0 = x / per * 32 * a.p_wr;
     it.rows = tokens * a.G;
-    it.kbeg = split * a.p_chunk;
-    it.kend = min(a.S, it.kbeg + a.p_chunk);
+    it.pbeg = split * a.p_chunk;
+    it.pend = min(a.S, it.pbeg + a.p_chunk);
     it.slot = a.o_splits + split;
     if (it.row0 >= it.rows) return;
     switch (a.p_wr) {
-      case 1: prefix_item<T, D, 1, false>(a, it, smem, s_pid, s_ml); break;
-      case 2: prefix_item<T, D, 2, false>(a, it, smem, s_pid, s_ml); break;
-      case 4: prefix_item<T, D, 4, false>(a, it, smem, s_pid, s_ml); break;
+      case 1: prefix_item<T, D, 1, kPromptItem>(a, it, smem, s_pid, s_ml); break;
+      case 2: prefix_item<T, D, 2, kPromptItem>(a, it, smem, s_pid, s_ml); break;
+      case 4: prefix_item<T, D, 4, kPromptItem>(a, it, smem, s_pid, s_ml); break;
       default:
-        if constexpr (Sh::kWaves == 8) prefix_item<T, D, 8, false>(a, it, smem, s_pid, s_ml);
+        if constexpr (NW >= 8) prefix_item<T, D, 8, kPromptItem>(a, it, smem, s_pid, s_ml);
         break;
     }
   } else {
@@ -656,7 +721,8 @@ prefix_attn_kernel(PrefixArgs a) {
     x /= a.Hk;
     const int split = x % a.o_splits;
     x /= a.o_splits;
-    const int tile = x % a.o_tiles, b = x / a.o_tiles;
+    // (late rows see most: they go first)
+    const int tile = a.o_tiles - 1 - x % a.o_tiles, b = x / a.o_tiles;
     int c0 = b, c1 = b + 1;
     if (a.cu) {
       c0 = min(max(a.cu[b], 0), tokens);
@@ -669,26 +735,41 @@ prefix_attn_kernel(PrefixArgs a) {
     if (it.row0 >= it.rows) return;
     const int chunk = own_chunk(len, a.o_splits);
     it.lim0 = len - n + 1;
-    it.kbeg = min((int64_t)split * chunk, (int64_t)len);
+    it.obeg = min((int64_t)split * chunk, (int64_t)len);
     const int last = min(it.row0 + 32 * a.o_wr, it.rows) - 1;   // the tile's row that sees most
-    it.kend = min(min(it.kbeg + chunk, len), max(0, it.lim0 + last / a.G));
+    it.oend = min(min(it.obeg + chunk, len), max(0, it.lim0 + last / a.G));
     it.table = a.tables + b * a.t_sb;
     it.slot = split;
-    if (it.kbeg >= it.kend) return;
+    if (a.both) {
+      it.oend = min(len, max(0, it.lim0 + last / a.G));
+      it.pend = a.prefix_lens ? min(max(a.prefix_lens[b], 0), a.S) : a.S;
+      switch (a.o_wr) {
+        case 1: prefix_item<T, D, 1, kBothItem>(a, it, smem, s_pid, s_ml); break;
+        case 2: prefix_item<T, D, 2, kBothItem>(a, it, smem, s_pid, s_ml); break;
+        case 4: prefix_item<T, D, 4, kBothItem>(a, it, smem, s_pid, s_ml); break;
+        default:
+          if constexpr (NW >= 8) prefix_item<T, D, 8, kBothItem>(a, it, smem, s_pid, s_ml);
+          break;
+      }
+      return;
+    }
+    if (it.obeg >= it.oend) return;
     switch (a.o_wr) {
-      case 1: prefix_item<T, D, 1, true>(a, it, smem, s_pid, s_ml); break;
-      case 2: prefix_item<T, D, 2, true>(a, it, smem, s_pid, s_ml); break;
-      case 4: prefix_item<T, D, 4, true>(a, it, smem, s_pid, s_ml); break;
+      case 1: prefix_item<T, D, 1, kOwnItem>(a, it, smem, s_pid, s_ml); break;
+      case 2: prefix_item<T, D, 2, kOwnItem>(a, it, smem, s_pid, s_ml); break;
+      case 4: prefix_item<T, D, 4, kOwnItem>(a, it, smem, s_pid, s_ml); break;
       default:
-        if constexpr (Sh::kWaves == 8) prefix_item<T, D, 8, true>(a, it, smem, s_pid, s_ml);
+        if constexpr (NW >= 8) prefix_item<T, D, 8, kOwnItem>(a, it, smem, s_pid, s_ml);
         break;
     }
   }
 }
 
-// Joins the partials of every query row: grid m_tiles tiles of kMergeRows rows
-// of each request, D / 4 threads a row.  A partial exists where the row sees
-// keys of its range, and where it does not the row has nothing there.
+// Joins the partials of every query row: grid m_tiles tiles of rows of each
+// request, D / 4 threads a row.  A partial exists where the row sees keys of
+// its range, and where it does not the row has nothing there.  The threads of a
+// row take a partial's (max, sum) each, so that all of them are one load deep;
+// then the outputs' loads, four dimensions a thread, go out eight at a time.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
   constexpr int kVec = D / 4, kRows = 256 / kVec;
@@ -700,41 +781,51 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
     c1 = min(max(a.cu[b + 1], c0), tokens);
   }
   const int n = c1 - c0, len = min(max(a.lens[b], 0), a.T << a.lp);
-  const int i = tile * kRows + threadIdx.x / kVec, dim = threadIdx.x % kVec * 4;
+  const int j = threadIdx.x % kVec, dim = 4 * j;
+  const int i = tile * kRows + threadIdx.x / kVec;
   const int t = i / a.Hq, h = i - t * a.Hq;
-  if (t >= min(n, a.max_new)) return;
+  if (t >= min(n, a.max_new)) return;   // (a row's threads together)
   const int S = a.prefix_lens ? min(max(a.prefix_lens[b], 0), a.S) : a.S;
   const int own = max(0, len - n + 1 + t), chunk = own_chunk(len, a.o_splits);
-  const int n_own = (min(own, len) + chunk - 1) / chunk, n_pre = a.p_splits ? (S + a.p_chunk - 1) / a.p_chunk : 0;
+  const int n_own = (own + chunk - 1) / chunk, n_pre = a.p_splits ? (S + a.p_chunk - 1) / a.p_chunk : 0;
   const int64_t rows_all = (int64_t)a.N * a.Hq, ridx = (int64_t)(c0 + t) * a.Hq + h;
   const int count = n_own + n_pre;
-  auto slot = [&](int s) { return s < n_own ? s : a.o_splits + s - n_own; };
+  // partial s of the row: the own ones first, then the prompt's
+  auto at = [&](int s) { return (s < n_own ? s : a.o_splits + s - n_own) * rows_all + ridx; };
+  typedef float floatx2 __attribute__((ext_vector_type(2)));
   float M = -INFINITY;
-  for (int s = 0; s < count; ++s) M = fmaxf(M, a.part_ml[(slot(s) * rows_all + ridx) * 2]);
+  for (int s = j; s < count; s += kVec) M = fmaxf(M, a.part_ml[at(s) * 2]);
+#pragma unroll
+  for (int o = kVec / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
   float L = 0.f;
   floatx4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int s = 0; s < count; ++s) {
-    const int64_t at = slot(s) * rows_all + ridx;
-    const float m = a.part_ml[at * 2], l = a.part_ml[at * 2 + 1];
-    const floatx4 o = *reinterpret_cast<const floatx4*>(a.part_o + at * D + dim);
-    const float w = m == -INFINITY ? 1.f : exp2_hw(m - M);   // (sums without a max are 0, or NaN)
-    L += l * w;
-    x += o * w;
+  for (int s0 = 0; s0 < count; s0 += kVec) {
+    const int mine = min(s0 + j, count - 1);
+    const floatx2 ml = *reinterpret_cast<const floatx2*>(a.part_ml + at(mine) * 2);
+    const float w = ml[0] == -INFINITY ? 1.f : exp2_hw(ml[0] - M);   // (sums without a max are 0, or NaN)
+    if (s0 + j < count) L += ml[1] * w;
+    const int todo = min(kVec, count - s0);
+    for (int k0 = 0; k0 < todo; k0 += 8) {
+      floatx4 o[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        o[k] = *reinterpret_cast<const floatx4*>(a.part_o + at(s0 + min(k0 + k, todo - 1)) * D + dim);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float wk = __shfl(w, (k0 + k) % kVec, kVec);
+        if (k0 + k < todo) x += o[k] * wk;
+      }
+    }
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  T* out = reinterpret_cast<T*>(a.out + (c0 + t) * a.o_sn + h * a.o_sh) + dim;
-  typedef T outx4 __attribute__((ext_vector_type(4)));
-  *reinterpret_cast<outx4*>(out) =
-      outx4{from_f32<T>(x[0] * inv), from_f32<T>(x[1] * inv), from_f32<T>(x[2] * inv), from_f32<T>(x[3] * inv)};
-  if (a.lse && dim == 0)
-    a.lse[(c0 + t) * a.l_sn + h * a.l_sh] = L == 0.f ? -INFINITY : (M + __log2f(L)) * 0.6931471805599453f;
+#pragma unroll
+  for (int o = kVec / 2; o > 0; o >>= 1) L += __shfl_xor(L, o, 64);
+  finish_row<T>(a, c0 + t, h, dim, x, M, L);
 }
 
 template <typename T, int D>
 void launch_prefix_d(const PrefixArgs& a, int64_t items, hipStream_t s) {
-  prefix_attn_kernel<T, D><<<(unsigned)items, PrefixShape<T, D>::kWaves * 64, 0, s>>>(a);
-  prefix_merge_kernel<T, D><<<(unsigned)(a.B * a.m_tiles), 256, 0, s>>>(a);
+  prefix_attn_kernel<T, D><<<(unsigned)items, PrefixShape<T, D>::NW * 64, 0, s>>>(a);
+  if (!a.both) prefix_merge_kernel<T, D><<<(unsigned)(a.B * a.m_tiles), 256, 0, s>>>(a);
 }
 
 template <typename T>

@@ -536,14 +536,16 @@ def test_lengths_past_the_table_are_cut():
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(DTYPES))
 def test_rows_behind_the_last_request_stay(dtype):
-    c = to_dev(paged_case(dtype, [40, 20], [7, 3], prefix=33))
+    host = paged_case(dtype, [40, 20], [7, 3], prefix=33)
+    c = to_dev(host)
     q = torch.full((25, 8, 64), math.nan, dtype=DTYPES[dtype], device="cuda")
     q[:10] = c["q"]
-    want = attend(c)
     out = torch.full((25, 2, 8, 64), 7.0, dtype=DTYPES[dtype], device="cuda")[:, 1]
     c["q"] = q
     got = attend(c, out=out)
-    assert got.data_ptr() == out.data_ptr() and torch.equal(out[:10], want) and (out[10:] == 7).all()
+    # (a larger token batch may be split otherwise: the same sums in another order, within the bound)
+    check_attention(out[:10], want_attention(host), DTYPES[dtype])
+    assert got.data_ptr() == out.data_ptr() and (out[10:] == 7).all()
 
 
 @pytest.mark.gpu
