@@ -16,42 +16,48 @@ constexpr int kCus = 256;
 
 // How a call is laid out over workgroups.
 struct PrefixPlan {
-  int p_wr, p_tiles, p_splits, p_chunk, o_wr, o_tiles, o_splits, m_tiles, both;
+  int p_rows, p_tiles, p_splits, p_chunk, o_rows, o_tiles, o_splits, m_tiles, m_sub, both;
   int64_t items, slots;
 };
 
-// Waves that share keys: as many as 32 rows each fill.
-int rows_waves(int64_t rows, int waves) {
-  int wr = 1;
-  while (wr < waves && rows > 32 * wr) wr *= 2;
-  return wr;
+// Query rows of a tile: as many as there are, up to 32 for each wave.
+int tile_rows(int64_t rows, int waves) {
+  int n = 16;
+  while (n < 32 * waves && rows > n) n *= 2;
+  return n;
 }
 
 // Times of a workgroup, in ns, as measured at head dimension 128 and 2-byte
-// types: kWgNs of its own (arguments, first loads, the waves' join), and a key's.
+// types: kWgNs of its own (arguments, first loads, the waves' join), and a key's; kSweepNs of a
+// second run of keys, kJoinNs of the partials' join.
 // One CU streams about 40 GB/s, all together kHbm; products of 32 WR rows take
 // the rest (30 ns a key of 256 rows).
-constexpr double kWgNs = 7000, kCuGBs = 40, kHbmGBs = 5000;
+constexpr double kWgNs = 6500, kSweepNs = 3500, kJoinNs = 4500, kCuGBs = 40, kHbmGBs = 5000;
 
 PrefixPlan plan_prefix(const hc_prefix_attn_args* x) {
   PrefixPlan p{};
   const int64_t es = dtype_size((int)x->dtype), G = x->Hq / x->Hk, rows = x->N * G, most = std::min(x->max_new, x->N);
   const int waves = x->D * es >= 512 ? 4 : 8;
   const double key_bytes = 2.0 * (double)(x->D * es);
-  auto key_ns = [&](int wr) { return std::max(key_bytes / kCuGBs, 3.75 * wr * 8 / waves * (double)(x->D * es * es) / 512); };
-  p.o_wr = rows_waves(most * G, waves);
-  p.o_tiles = (int)cdiv(most * G, 32 * p.o_wr);
+  auto key_ns = [&](int n) { return std::max(key_bytes / kCuGBs, 0.117 * n * 8 / waves * (double)(x->D * es * es) / 512); };
+  p.o_rows = tile_rows(most * G, waves);
+  p.o_tiles = (int)cdiv(most * G, p.o_rows);
   // Own items: a request's keys are split only as far as it takes to give every
   // CU some.  Their lengths are on the device; half of what the table holds is
   // taken for the mean.
   const int64_t units = x->B * x->Hk * p.o_tiles, longest = x->table_width * x->page_size;
   p.o_splits = (int)std::max<int64_t>(1, std::min<int64_t>({cdiv((int64_t)kCus / 2, units), cdiv(longest, (int64_t)256), 64}));
   const double own_keys = 0.5 * (double)longest / p.o_splits;
-  const double own_n = (double)units * p.o_splits, own_ns = kWgNs + own_keys * key_ns(p.o_wr);
+  // (tiles that hold rows: a request's last one is half full)
+  const double tiles = std::min((double)(x->B * p.o_tiles), (double)rows / p.o_rows + 0.5 * (double)x->B);
+  const double own_n = tiles * (double)(x->Hk * p.o_splits), own_ns = kWgNs + own_keys * key_ns(p.o_rows);
+  double two = own_n * own_ns / kCus;   // prompt and own items, and the join
   if (x->prefix_rows > 0) {
-    p.p_wr = rows_waves(rows, waves);
-    p.p_tiles = (int)cdiv(rows, 32 * p.p_wr);
-    const int64_t bn = p.p_wr == waves ? 64 : std::max(128, 32 * (waves / p.p_wr)), units_p = p.p_tiles * x->Hk;
+    p.p_rows = tile_rows(rows, waves);
+    p.p_tiles = (int)cdiv(rows, p.p_rows);
+    // (a tile's keys, as in the kernel)
+    const int wk = waves * 32 / std::max(32, p.p_rows);
+    const int64_t bn = wk * (wk <= waves / 4 ? 64 : 32), units_p = p.p_tiles * x->Hk;
     // Prompt items go first, and the own ones on the CUs they leave.  With s
     // splits they take t; by then each CU left has done t / own_ns own items,
     // and what remains of them runs on all CUs (or at the memory's rate).
@@ -60,7 +66,7 @@ PrefixPlan plan_prefix(const hc_prefix_attn_args* x) {
       const int64_t chunk = cdiv(cdiv(x->prefix_rows, s), bn) * bn, splits = cdiv(x->prefix_rows, chunk);
       const double n = (double)(units_p * splits), rounds = std::ceil(n / kCus);
       const double left = std::max(0.0, kCus - n);
-      double t = rounds * (kWgNs + (double)chunk * key_ns(p.p_wr));
+      double t = rounds * (kWgNs + (double)chunk * key_ns(p.p_rows));
       const double done = std::min(own_n, left * std::floor(t / own_ns));
       t = std::max(t, (n * (double)chunk + done * own_keys) * key_bytes / kHbmGBs);
       const double rest = own_n - done;
@@ -73,8 +79,23 @@ PrefixPlan plan_prefix(const hc_prefix_attn_args* x) {
       }
       if (chunk == bn) break;
     }
+    two = best;
   }
-  p.m_tiles = (int)cdiv(most * x->Hq * (x->D / 4), (int64_t)256);
+  two += kJoinNs + (double)(p.o_splits * rows * x->Hk * x->D * 8) / kHbmGBs;
+  // Or each own item takes the prompt as well: no partials, but the prompt once
+  // for every request's tile.  (Requests' own prompts of up to 512 tokens behind
+  // 64 rows: 94 us -> 61.  Of 1024 behind 8192, where the estimates are close:
+  // 802 us apart, 963 together.)
+  const double both = std::ceil(tiles * (double)x->Hk / kCus) *
+                      (kWgNs + (x->prefix_rows > 0 ? kSweepNs : 0) +
+                       ((double)x->prefix_rows + 0.5 * (double)longest) * key_ns(p.o_rows));
+  if ((p.both = both < 0.9 * two)) {
+    p.p_tiles = p.p_splits = 0;
+    p.o_splits = 1;
+  }
+  const int64_t vec = x->D / 4;   // threads of a row's group
+  p.m_sub = x->D == 128 && x->B * cdiv(most * x->Hq * vec, (int64_t)256) < 2 * kCus && p.p_splits + p.o_splits >= 8 ? kMergeSub : 1;
+  p.m_tiles = (int)cdiv(most * x->Hq * vec * p.m_sub, (int64_t)256);
   p.items = (int64_t)p.p_tiles * x->Hk * p.p_splits + units * p.o_splits;
   p.slots = p.p_splits + p.o_splits;
   return p;
@@ -168,9 +189,9 @@ extern "C" int hc_prefix_attn(const hc_prefix_attn_args* x, void* stream) {
   a.D = (int)x->D; a.S = (int)x->prefix_rows; a.T = (int)x->table_width; a.lp = page_shift(x->page_size);
   a.num_pages = (int)x->num_pages;
   a.max_new = (int)std::min<int64_t>(x->max_new, x->N);
-  a.p_wr = p.p_wr; a.p_tiles = p.p_tiles; a.p_splits = p.p_splits; a.p_chunk = p.p_chunk;
+  a.p_rows = p.p_rows; a.p_tiles = p.p_tiles; a.p_splits = p.p_splits; a.p_chunk = p.p_chunk;
   a.p_items = p.p_tiles * a.Hk * p.p_splits;
-  a.o_wr = p.o_wr; a.o_tiles = p.o_tiles; a.o_splits = p.o_splits; a.both = p.both; a.m_tiles = p.m_tiles;
+  a.o_rows = p.o_rows; a.o_tiles = p.o_tiles; a.o_splits = p.o_splits; a.both = p.both; a.m_tiles = p.m_tiles; a.m_sub = p.m_sub;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (dtype == HC_DTYPE_F16) launch_prefix<half_t>(a, p.items, s);
   else if (dtype == HC_DTYPE_BF16) launch_prefix<bf16_t>(a, p.items, s);

@@ -12,17 +12,18 @@
 //   * own items: (request, KV head, tile of its query rows, key range of its
 //     pages).
 // Each writes (max, sum, unnormalised output) of its rows for its keys, and a
-// second launch joins them.
+// second launch joins them.  Where the prompt is short, or absent, the own items
+// take it too and write their rows complete: one launch.
 //
 // A workgroup's NW waves are WR x WK: WR waves share the keys and take 32
-// query rows each, WK waves take different keys.  WR follows the rows there
-// are (32 to 32 NW a tile): a single request's few rows put every wave on keys
-// of its own.
-//   * Scores are K.Q^T (v_mfma_f32_32x32x16, fp32 inputs 32x32x2): a lane
-//     holds one query row's scores of 16 keys, so the row's running max and
-//     sum live in its two lanes, and its probabilities are, as they stand, the
-//     B operand of V^T.P^T: the product's order of keys is the score layout's
-//     (key (i & 3) + 8 (i / 4) + 4 (lane / 32) in register i), and V^T's
+// query rows each (16, where a tile has no more), WK waves take different keys.
+// WR follows the rows there are (16 to 32 NW a tile): a single request's few
+// rows put every wave on keys of its own.
+//   * Scores are K.Q^T (v_mfma_f32_32x32x16, fp32 inputs 32x32x2; 16x16x32 and
+//     16x16x4 for tiles of 16 rows): a lane holds one query row's scores of 16
+//     keys, so the row's running max and sum live in its two (four) lanes, and
+//     its probabilities are, as they stand, the B operand of V^T.P^T: the
+//     product's order of keys is the score layout's (index, below), and V^T's
 //     operand is read in that order, by LDS transpose reads (ds_read_b64_tr)
 //     for 2-byte types.  The output is transposed, too: a lane owns its
 //     query's column, and the rescale is a multiply by the lane's own factor.
@@ -75,16 +76,17 @@ struct PrefixArgs {
   float scale_log2;
   uint32_t q_and, q_xor;
   int N, B, Hq, Hk, G, D, S, T, lp, num_pages, max_new;
-  // prompt items: WR of their workgroups, row tiles, key splits and rows a
-  // split; own items: WR, row tiles and splits of one request
-  int p_wr, p_tiles, p_splits, p_chunk, p_items;
-  int o_wr, o_tiles, o_splits;
+  // prompt items: query rows of a tile, tiles, key splits and keys a split; own
+  // items: rows of a tile, tiles and splits of one request
+  int p_rows, p_tiles, p_splits, p_chunk, p_items;
+  int o_rows, o_tiles, o_splits;
   int both;   // own items take the prompt too: no prompt items, no partials
-  // merge: tiles of rows of one request
-  int m_tiles;
+  // merge: tiles of rows of one request, groups of threads a row
+  int m_tiles, m_sub;
 };
 
 constexpr float kLazy = 8.f;
+constexpr int kMergeSub = 8;    // groups of threads a row, where few rows have many partials
 constexpr int kPageIds = 2048;  // page numbers held in LDS at a time
 
 // NW waves a workgroup, one workgroup a CU (256 registers a lane, most of LDS):
@@ -109,12 +111,22 @@ __host__ __device__ __forceinline__ int own_chunk(int len, int splits) {
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// max / sum of a lane's value with lane ^ 32's
-__device__ __forceinline__ float half_max(float x) {
+// max / sum over a column's lanes (lane % RW)
+template <int RW>
+__device__ __forceinline__ float col_max(float x) {
+  if constexpr (RW == 16) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  }
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
-__device__ __forceinline__ float half_sum(float x) {
+template <int RW>
+__device__ __forceinline__ float col_sum(float x) {
+  if constexpr (RW == 16) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  }
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
@@ -149,28 +161,55 @@ __device__ __forceinline__ int fresh(int x) {
   return x;
 }
 
-template <typename T>
+// One product of RW x RW outputs: A's RW rows are keys (or dimensions of V), B's
+// RW columns query rows.  A lane holds column lane % RW; lanes / RW are its
+// groups.  Register i of an output is row index(i, group) of its block.
+template <typename T, int RW>
 struct Mma;
 template <>
-struct Mma<half_t> {
+struct Mma<half_t, 32> {
   typedef half8 frag;
-  __device__ static floatx16 mma(half8 a, half8 b, floatx16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-  }
+  typedef floatx16 out;
+  __device__ static out mma(frag a, frag b, out c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 template <>
-struct Mma<bf16_t> {
+struct Mma<half_t, 16> {
+  typedef half8 frag;
+  typedef floatx4 out;
+  __device__ static out mma(frag a, frag b, out c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Mma<bf16_t, 32> {
   typedef bf16x8 frag;
-  __device__ static floatx16 mma(bf16x8 a, bf16x8 b, floatx16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  typedef floatx16 out;
+  __device__ static out mma(frag a, frag b, out c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Mma<bf16_t, 16> {
+  typedef bf16x8 frag;
+  typedef floatx4 out;
+  __device__ static out mma(frag a, frag b, out c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+// (fp32: a fragment's four elements are four products of one element each)
+template <>
+struct Mma<float, 32> {
+  typedef floatx4 frag;
+  typedef floatx16 out;
+  __device__ static out one(float a, float b, out c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
+  __device__ static out mma(frag a, frag b, out c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = one(a[j], b[j], c);
+    return c;
   }
 };
 template <>
-struct Mma<float> {
-  typedef floatx4 frag;   // four products of two dimensions each
-  __device__ static floatx16 mma(floatx4 a, floatx4 b, floatx16 c) {
+struct Mma<float, 16> {
+  typedef floatx4 frag;
+  typedef floatx4 out;
+  __device__ static out one(float a, float b, out c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+  __device__ static out mma(frag a, frag b, out c) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    for (int j = 0; j < 4; ++j) c = one(a[j], b[j], c);
     return c;
   }
 };
@@ -198,13 +237,18 @@ __device__ __forceinline__ void finish_row(const PrefixArgs& a, int t, int h, in
     a.lse[t * a.l_sn + h * a.l_sh] = L == 0.f ? -INFINITY : (M + __log2f(L)) * 0.6931471805599453f;
 }
 
-template <typename T, int D, int WR, int kMode>
+// A workgroup's part: RW query rows a wave (16 where no more are there: half the
+// work and registers of 32), WR waves sharing the keys.
+template <typename T, int D, int RW, int WR, int kMode>
 __device__ __forceinline__ void prefix_item(const PrefixArgs& a, const Item& it, char* smem, int32_t* s_pid, float* s_ml) {
   using Sh = PrefixShape<T, D>;
+  typedef Mma<T, RW> M_;
+  typedef typename M_::frag frag;
+  typedef typename M_::out out_t;
   constexpr int NW = Sh::NW;
   constexpr int kRowB = Sh::kRowB, kPieces = Sh::kPieces, WK = NW / WR;
   constexpr int KT = WK <= NW / 4 ? 64 : 32;   // keys a wave takes of a tile
-  constexpr int KB = KT / 32, BN = WK * KT;
+  constexpr int KB = KT / RW, BN = WK * KT;
   constexpr int kStages = WR == 1 ? 1 : 2;
   constexpr int kRows = KT / WR;               // rows of a tile a wave loads
   constexpr int kPerLoad = 64 / kPieces;       // rows of one load
@@ -212,38 +256,38 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, const Item& it,
   constexpr bool kPartial = kRows < kPerLoad;  // a load's last lanes stay idle
   constexpr int kSt = BN * kRowB;              // bytes of a tile's K, or V
   static_assert(2 * kSt * kStages <= Sh::kLds, "tiles fit LDS");
-  constexpr int NB = (D + 31) / 32;            // blocks of 32 output dimensions
   constexpr bool kF32 = sizeof(T) == 4;
-  typedef typename Mma<T>::frag frag;
-  constexpr int NQ = kF32 ? D / 8 : (D + 15) / 16;
+  constexpr int kGroups = 64 / RW, kAcc = RW * RW / 64;
+  constexpr int NB = (D + RW - 1) / RW;        // blocks of RW output dimensions
+  constexpr int NQ = (kPieces + kGroups - 1) / kGroups;   // a piece a group and product
+  constexpr int kPk = 8 * kGroups;             // keys of an output product (2-byte types)
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int wr = wave % WR, wk = wave / WR;
-  const int col = lane & 31, half = lane >> 5;
+  const int col = lane % RW, grp = lane / RW;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+  auto index = [](int i, int g) { return RW == 32 ? (i & 3) + 8 * (i >> 2) + 4 * g : i + 4 * g; };
 
-  // ---- the wave's query rows
-  const int r = it.row0 + 32 * wr + col;
+  // ---- the wave's query rows (used, and so waited for, behind the first keys' loads)
+  const int r = it.row0 + RW * wr + col;
   const bool live = r < it.rows;
   const int tok = it.tok0 + (live ? r / a.G : 0);
   const int head = it.hk * a.G + (live ? r % a.G : 0);
-  typename Mma<T>::frag qf[NQ];
+  u32x4 qw[NQ];
   {
     const char* qp = a.q + tok * a.q_sn + head * a.q_sh;
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
-      u32x4 x = {0u, 0u, 0u, 0u};
-      if (live) x = ld16(qp + 32 * t + 16 * half);
-      x = (x & a.q_and) ^ a.q_xor;
-      qf[t] = __builtin_bit_cast(typename Mma<T>::frag, x);
+      qw[t] = u32x4{0u, 0u, 0u, 0u};
+      if (live && (kPieces % kGroups == 0 || kGroups * t + grp < kPieces)) qw[t] = ld16(qp + 16 * (kGroups * t + grp));
     }
   }
-  floatx16 acc[NB];
+  out_t acc[NB];
 #pragma unroll
   for (int d = 0; d < NB; ++d)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+    for (int i = 0; i < kAcc; ++i) acc[d][i] = 0.f;
   float m = -INFINITY, l = 0.f;
 
   // f(r) of row r: pieces of 16 rows with the same number lie on distinct
@@ -259,335 +303,330 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, const Item& it,
   // The keys [kbeg, kend) of the prompt or of the request's pages: the lane's
   // row sees those below lim, every row of the workgroup those below all.
   auto sweep = [&](auto own_keys, const int kbeg, const int kend, const int all, const int lim) {
-  constexpr bool kOwn = decltype(own_keys)::value;
-  // rows see different keys: a value that is not finite may have to reach some
-  // of them only
-  const bool ragged = all != kend;
-  const char* kbase = kOwn ? a.kg + it.hk * a.kg_sh : a.kp + it.hk * a.kp_sh;
-  const char* vbase = kOwn ? a.vg + it.hk * a.vg_sh : a.vp + it.hk * a.vp_sh;
-  // (a segment's first page may be entered in its middle)
-  const int seg_keys = kOwn ? ((kPageIds - 1) << min(a.lp, 12)) / BN * BN : 0x7fffffff;
-  for (int seg = kbeg, send; seg < kend; seg = send) {
-    send = kend - seg > seg_keys ? seg + seg_keys : kend;
-    bool bad_pages = false;
-    const int page0 = seg >> a.lp;
-    if constexpr (kOwn) {
-      if (seg != kbeg) __syncthreads();   // the last segment's pages are read
-      int bad = 0;
-      const int n = ((send - 1) >> a.lp) - page0 + 1;
-      for (int i = threadIdx.x; i < n; i += NW * 64) {
-        const int p = it.table[page0 + i];
-        const bool ok = (uint32_t)p < (uint32_t)a.num_pages;
-        s_pid[i] = ok ? p : -1;
-        bad |= !ok;
+    constexpr bool kOwn = decltype(own_keys)::value;
+    // rows see different keys: a value that is not finite may have to reach some
+    // of them only
+    const bool ragged = all != kend;
+    const char* kbase = kOwn ? a.kg + it.hk * a.kg_sh : a.kp + it.hk * a.kp_sh;
+    const char* vbase = kOwn ? a.vg + it.hk * a.vg_sh : a.vp + it.hk * a.vp_sh;
+    // (a segment's first page may be entered in its middle)
+    const int seg_keys = kOwn ? ((kPageIds - 1) << min(a.lp, 12)) / BN * BN : 0x7fffffff;
+    for (int seg = kbeg, send; seg < kend; seg = send) {
+      send = kend - seg > seg_keys ? seg + seg_keys : kend;
+      bool bad_pages = false;
+      const int page0 = seg >> a.lp;
+      if constexpr (kOwn) {
+        if (seg != kbeg) __syncthreads();   // the last segment's pages are read
+        int bad = 0;
+        const int n = ((send - 1) >> a.lp) - page0 + 1;
+        for (int i = threadIdx.x; i < n; i += NW * 64) {
+          const int p = it.table[page0 + i];
+          const bool ok = (uint32_t)p < (uint32_t)a.num_pages;
+          s_pid[i] = ok ? p : -1;
+          bad |= !ok;
+        }
+        int* s_bad = reinterpret_cast<int*>(s_ml);
+        bad = __any(bad);
+        if (lane == 0) s_bad[wave] = bad;
+        __syncthreads();   // (also: the tiles of the keys before are read)
+        int any = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) any |= s_bad[w];
+        bad_pages = __builtin_amdgcn_readfirstlane(any) != 0;
       }
-      int* s_bad = reinterpret_cast<int*>(s_ml);
-      bad = __any(bad);
-      if (lane == 0) s_bad[wave] = bad;
-      __syncthreads();   // (also: the tiles of the keys before are read)
-      int any = 0;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) any |= s_bad[w];
-      bad_pages = __builtin_amdgcn_readfirstlane(any) != 0;
-    }
 
-    // asynchronous loads of the wave's rows of the tile at key0: consecutive
-    // keys, one address and the lanes' offsets where they are in one page
-    auto issue = [&](int key0, int stage, bool v) {
-      const int piece = lane % kPieces, sub = lane / kPieces;
-      const uint32_t dst = lds0 + (uint32_t)((stage * 2 + (v ? 1 : 0)) * kSt + (wk * KT + wr * kRows) * kRowB);
-      const int64_t ss = kOwn ? (v ? a.vg_ss : a.kg_ss) : (v ? a.vp_ss : a.kp_ss);
-      const char* base = v ? vbase : kbase;
-      const int first = key0 + wk * KT + wr * kRows;
-      // (f of a sum of rows with distinct bits is the xor of theirs)
-      const uint32_t at = 16 * (piece ^ swz(wr * kRows + sub));
-      if (first + kRows <= send && (!kOwn || (1 << a.lp) >= kRows)) {
-        if constexpr (kOwn) {
-          const int pid = __builtin_amdgcn_readfirstlane(s_pid[(first >> a.lp) - page0]);
-          base += (int64_t)max(pid, 0) * (v ? a.vg_sp : a.kg_sp) + (int64_t)(first & ((1 << a.lp) - 1)) * ss;
-        } else {
-          base += (int64_t)first * ss;
-        }
-        const uint32_t rows = (uint32_t)sub * (uint32_t)ss;
-        if (!kPartial || lane < kRows * kPieces) {
+      // asynchronous loads of the wave's rows of the tile at key0: consecutive
+      // keys, one address and the lanes' offsets where they are in one page
+      auto issue = [&](int key0, int stage, bool v) {
+        const int piece = lane % kPieces, sub = lane / kPieces;
+        const uint32_t dst = lds0 + (uint32_t)((stage * 2 + (v ? 1 : 0)) * kSt + (wk * KT + wr * kRows) * kRowB);
+        const int64_t ss = kOwn ? (v ? a.vg_ss : a.kg_ss) : (v ? a.vp_ss : a.kp_ss);
+        const char* base = v ? vbase : kbase;
+        const int first = key0 + wk * KT + wr * kRows;
+        // (f of a sum of rows with distinct bits is the xor of theirs)
+        const uint32_t at = 16 * (piece ^ swz(wr * kRows + sub));
+        if (first + kRows <= send && (!kOwn || (1 << a.lp) >= kRows)) {
+          if constexpr (kOwn) {
+            const int pid = __builtin_amdgcn_readfirstlane(s_pid[(first >> a.lp) - page0]);
+            base += (int64_t)max(pid, 0) * (v ? a.vg_sp : a.kg_sp) + (int64_t)(first & ((1 << a.lp) - 1)) * ss;
+          } else {
+            base += (int64_t)first * ss;
+          }
+          const uint32_t rows = (uint32_t)sub * (uint32_t)ss;
+          if (!kPartial || lane < kRows * kPieces) {
 #pragma unroll
-          for (int j = 0; j < kLoads; ++j)
-            load_to_lds(base + j * kPerLoad * ss, (at ^ (16 * swz(j * kPerLoad))) + rows, dst + j * 1024);
+            for (int j = 0; j < kLoads; ++j)
+              load_to_lds(base + j * kPerLoad * ss, (at ^ (16 * swz(j * kPerLoad))) + rows, dst + j * 1024);
+          }
+        } else {
+#pragma unroll 1
+          for (int j = 0; j < kLoads; ++j) {
+            // keys past the end load the last one's row (zeroed below)
+            const int key = min(first + j * kPerLoad + sub, send - 1);
+            const char* p = base;
+            if constexpr (kOwn) {
+              const int pid = max(s_pid[(key >> a.lp) - page0], 0);
+              p += (int64_t)pid * (v ? a.vg_sp : a.kg_sp) + (int64_t)(key & ((1 << a.lp) - 1)) * ss;
+            } else {
+              p += (int64_t)key * ss;
+            }
+            if (!kPartial || lane < kRows * kPieces) load_to_lds(p + (at ^ (16 * swz(j * kPerLoad))), dst + j * 1024);
+          }
         }
-      } else {
+      };
+      auto hidden = [&](int key) {   // a key of the segment's tiles that nobody attends
+        if (key >= send) return true;
+        if constexpr (kOwn) return bad_pages && s_pid[(key >> a.lp) - page0] < 0;
+        return false;
+      };
+      // zero the wave's loaded rows of keys nobody attends
+      auto clear = [&](int key0, int stage, bool v) {
+        const int ln = fresh(lane);
 #pragma unroll 1
         for (int j = 0; j < kLoads; ++j) {
-          // keys past the end load the last one's row (zeroed below)
-          const int key = min(first + j * kPerLoad + sub, send - 1);
-          const char* p = base;
-          if constexpr (kOwn) {
-            const int pid = max(s_pid[(key >> a.lp) - page0], 0);
-            p += (int64_t)pid * (v ? a.vg_sp : a.kg_sp) + (int64_t)(key & ((1 << a.lp) - 1)) * ss;
-          } else {
-            p += (int64_t)key * ss;
+          const int row = wr * kRows + j * kPerLoad + ln / kPieces;
+          if ((!kPartial || ln < kRows * kPieces) && hidden(key0 + wk * KT + row))
+            st16(smem + (stage * 2 + (v ? 1 : 0)) * kSt + (wk * KT + row) * kRowB + (ln % kPieces) * 16,
+                 u32x4{0u, 0u, 0u, 0u});
+        }
+      };
+      // the order of a phase's LDS reads and products: operands a few products ahead
+      auto order = [](auto products, auto reads, auto ahead, auto id) {
+        constexpr int kN = decltype(products)::value, kR = decltype(reads)::value, kId = decltype(id)::value;
+        constexpr int kA = kN < decltype(ahead)::value ? kN : decltype(ahead)::value;
+        __builtin_amdgcn_sched_group_barrier(0x100, kR * kA, kId);
+        static_for<kN - kA>([](auto) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, kId);
+          __builtin_amdgcn_sched_group_barrier(0x100, kR, kId);
+        });
+        __builtin_amdgcn_sched_group_barrier(0x8, kA, kId);
+      };
+      using std::integral_constant;
+
+      int tile = seg;
+      const int whole = bad_pages ? seg : min(all, send);
+      // one tile; kAll: every row sees all of its keys
+      auto do_tile = [&](int n, auto all_see) {
+        constexpr bool kAll = decltype(all_see)::value;
+        const int stage = kStages == 1 ? 0 : (n & 1);
+        const bool more = tile + BN < send;
+        const bool edge = !kAll && (tile + BN > send || bad_pages);
+        if constexpr (WR == 1) {
+          // the wave's own rows: its V loads (kLoads of them) may be in flight
+          vm_wait<kLoads>();
+          if (edge) clear(tile, 0, false);
+        } else {
+          vm_wait<0>();
+          if (edge) {
+            clear(tile, stage, false);
+            clear(tile, stage, true);
           }
-          if (!kPartial || lane < kRows * kPieces) load_to_lds(p + (at ^ (16 * swz(j * kPerLoad))), dst + j * 1024);
-        }
-      }
-    };
-    auto hidden = [&](int key) {   // a key of the segment's tiles that nobody attends
-      if (key >= send) return true;
-      if constexpr (kOwn) return bad_pages && s_pid[(key >> a.lp) - page0] < 0;
-      return false;
-    };
-    // zero the wave's loaded rows of keys nobody attends
-    auto clear = [&](int key0, int stage, bool v) {
-      const int ln = fresh(lane);
-#pragma unroll 1
-      for (int j = 0; j < kLoads; ++j) {
-        const int row = wr * kRows + j * kPerLoad + ln / kPieces;
-        if ((!kPartial || ln < kRows * kPieces) && hidden(key0 + wk * KT + row))
-          st16(smem + (stage * 2 + (v ? 1 : 0)) * kSt + (wk * KT + row) * kRowB + (ln % kPieces) * 16,
-               u32x4{0u, 0u, 0u, 0u});
-      }
-    };
-
-    // scores of the wave's keys of a tile
-    auto qk = [&](const char* ks, floatx16 (&s)[KB]) {
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
-#pragma unroll
-      for (int t = 0; t < NQ; ++t)
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          const int row = 32 * kb + col;
-          const u32x4 x = ld16(ks + row * kRowB + (((2 * t + half) ^ swz(row)) << 4));
-          s[kb] = Mma<T>::mma(__builtin_bit_cast(frag, x), qf[t], s[kb]);
-        }
-    };
-    // scores to probabilities (against the row's reference), and their sum
-    auto softmax = [&](floatx16 (&s)[KB]) {
-      float t = s[0][0], u = s[0][1];
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          t = fmaxf(fmaxf(t, s[kb][i]), s[kb][i + 1]);
-          u = fmaxf(fmaxf(u, s[kb][i + 2]), s[kb][i + 3]);
-        }
-      t = half_max(fmaxf(t, u)) * a.scale_log2;
-      const bool bump = t > m + kLazy;
-      if (__any(bump)) {
-        const float mn = bump ? t : m;
-        const float alpha = bump ? exp2_hw(m - mn) : 1.f;
-        m = mn;
-        l *= alpha;
-#pragma unroll
-        for (int d = 0; d < NB; ++d)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
-      }
-      const float ref = m == -INFINITY ? 0.f : m;   // (a row that has seen nothing yet: its terms are 0)
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[kb][i] = exp2_hw(__builtin_fmaf(s[kb][i], a.scale_log2, -ref));
-          sum[i & 3] += s[kb][i];
-        }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    };
-    // probabilities of 16 keys as a product's operand
-    auto pack = [&](const floatx16 (&s)[KB], frag (&p)[2 * KB]) {
-#pragma unroll
-      for (int h = 0; h < 2 * KB; ++h)
-#pragma unroll
-        for (int j = 0; j < 16 / (int)sizeof(T); ++j) p[h][j] = from_f32<T>(s[h / 2][8 * (h & 1) + j]);
-    };
-    // output of the wave's keys of a tile (2-byte types); with zero, of zeros
-    auto pv = [&](const char* vs, const frag (&p)[2 * KB], auto may_zero, bool zero) {
-      typedef __attribute__((address_space(3))) shortx4 lds4;
-#pragma unroll
-      for (int h = 0; h < 2 * KB; ++h) {
-        const int row = 16 * h + 4 * half + ((lane & 15) >> 2);
-#pragma unroll
-        for (int d = 0; d < NB; ++d) {
-          // dimensions past D (16) read the row's first ones; their output is not used
-          const int dim = (D % 32 == 0 ? 32 * d + 16 * ((lane >> 4) & 1) : 0) + 4 * (lane & 3);
-          union {
-            shortx4 h[2];
-            u32x4 w;
-          } u;
-          u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (lds4*)(vs + row * kRowB + (((dim >> 3) ^ swz(row)) << 4) + (dim & 4) * 2));
-          u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (lds4*)(vs + (row + 8) * kRowB + (((dim >> 3) ^ swz(row + 8)) << 4) + (dim & 4) * 2));
-          frag f = p[h];
-          if constexpr (decltype(may_zero)::value) {
-            const uint32_t mask = zero ? 0u : ~0u;
-            u.w &= mask;
-            f = __builtin_bit_cast(frag, __builtin_bit_cast(u32x4, f) & mask);
+          __syncthreads();
+          if (more) {
+            issue(tile + BN, stage ^ 1, false);
+            issue(tile + BN, stage ^ 1, true);
           }
-          acc[d] = Mma<T>::mma(__builtin_bit_cast(frag, u.w), f, acc[d]);
         }
-      }
-    };
-    // the order of a phase's LDS reads and products: operands a few products ahead
-    auto order = [](auto products, auto reads, auto ahead, auto id) {
-      constexpr int kN = decltype(products)::value, kR = decltype(reads)::value, kId = decltype(id)::value;
-      constexpr int kA = kN < decltype(ahead)::value ? kN : decltype(ahead)::value;
-      __builtin_amdgcn_sched_group_barrier(0x100, kR * kA, kId);
-      static_for<kN - kA>([](auto) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, kId);
-        __builtin_amdgcn_sched_group_barrier(0x100, kR, kId);
-      });
-      __builtin_amdgcn_sched_group_barrier(0x8, kA, kId);
-    };
-    using std::integral_constant;
-    typedef integral_constant<int, NQ * KB> QkProducts;
-    typedef integral_constant<int, 2 * KB * NB> PvProducts;
-    auto tile_k = [&](int stage) { return smem + stage * 2 * kSt + wk * KT * kRowB; };
+        const char* ks = smem + stage * 2 * kSt + wk * KT * kRowB;
+        const char* vs = ks + kSt;
+        const int key0 = tile + wk * KT;
 
-    int tile = seg;
-    const int whole = bad_pages ? seg : min(all, send);
-    // one tile; kAll: every row sees all of its keys
-    auto do_tile = [&](int n, auto all_see) {
-      constexpr bool kAll = decltype(all_see)::value;
-      const int stage = kStages == 1 ? 0 : (n & 1);
-      const bool more = tile + BN < send;
-      const bool edge = !kAll && (tile + BN > send || bad_pages);
-      if constexpr (WR == 1) {
-        // the wave's own rows: its V loads (kLoads of them) may be in flight
-        vm_wait<kLoads>();
-        if (edge) clear(tile, 0, false);
-      } else {
-        vm_wait<0>();
-        if (edge) {
-          clear(tile, stage, false);
-          clear(tile, stage, true);
-        }
-        __syncthreads();
-        if (more) {
-          issue(tile + BN, stage ^ 1, false);
-          issue(tile + BN, stage ^ 1, true);
-        }
-      }
-      const char* ks = tile_k(stage);
-      const char* vs = ks + kSt;
-      const int key0 = tile + wk * KT;
-
-      floatx16 s[KB];
-      qk(ks, s);
-      if constexpr (kAll && !kF32)
-        order(QkProducts{}, integral_constant<int, 1>{}, integral_constant<int, 6>{}, integral_constant<int, 0>{});
-      if constexpr (WR == 1) {
-        if (more) {
-          lds_wait();   // the tile's reads are done
-          issue(tile + BN, 0, false);
-        }
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      if constexpr (!kAll) {
-        const int first = key0 + 4 * fresh(half);
+        // ---- scores
+        out_t s[KB];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int key = first + 32 * kb + (i & 3) + 8 * (i >> 2);
-            bool see = key < lim;
-            if (bad_pages) see = see && !hidden(key);
-            s[kb][i] = see ? s[kb][i] : -INFINITY;
-          }
-      }
-      softmax(s);
-      if constexpr (WR == 1) {
-        if (more) vm_wait<kLoads>(); else vm_wait<0>();
-        if (edge) clear(tile, 0, true);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      bool slow = false;
-      if (!kAll && ragged) {
-        // a value that is not finite in this tile?
-        uint32_t odd = 0;
-        for (int i = fresh(lane); i < KT * kPieces; i += 64) {
-          const u32x4 x = ld16(vs + 16 * i);
+          for (int i = 0; i < kAcc; ++i) s[kb][i] = 0.f;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            if constexpr (kF32) {
-              odd |= (x[w] & 0x7f800000u) == 0x7f800000u;
-            } else {
-              constexpr uint32_t kExp = std::is_same<T, half_t>::value ? 0x7c00u : 0x7f80u;
-              odd |= (x[w] & kExp) == kExp;
-              odd |= ((x[w] >> 16) & kExp) == kExp;
-            }
+        for (int t = 0; t < NQ; ++t)
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) {
+            const int row = RW * kb + col;
+            u32x4 x = ld16(ks + row * kRowB + ((((kGroups * t + grp) % kPieces) ^ swz(row)) << 4));
+            if constexpr (kPieces % kGroups != 0)
+              if (kGroups * t + grp >= kPieces) x = u32x4{0u, 0u, 0u, 0u};
+            s[kb] = M_::mma(__builtin_bit_cast(frag, x), __builtin_bit_cast(frag, qw[t]), s[kb]);
+          }
+        if constexpr (kAll && !kF32)
+          order(integral_constant<int, NQ * KB>{}, integral_constant<int, 1>{}, integral_constant<int, 6>{},
+                integral_constant<int, 0>{});
+        if constexpr (WR == 1) {
+          if (more) {
+            lds_wait();   // the tile's reads are done
+            issue(tile + BN, 0, false);
           }
         }
-        slow = __any(odd);
-      }
-      if constexpr (kF32) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int row = 32 * kb + (i & 3) + 8 * (i >> 2) + 4 * half;
-#pragma unroll
-            for (int d = 0; d < NB; ++d) {
-              const int dim = min(32 * d + col, D - 1);   // (outputs past D are not used)
-              float v = *reinterpret_cast<const float*>(vs + row * kRowB + (((dim >> 2) ^ swz(row)) << 4) + (dim & 3) * 4);
-              float p = s[kb][i];
-              if constexpr (!kAll) {
-                v = slow ? 0.f : v;
-                p = slow ? 0.f : p;
-              }
-              acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p, acc[d], 0, 0, 0);
-            }
-          }
-      } else {
-        frag p[2 * KB];
-        pack(s, p);
-        pv(vs, p, integral_constant<bool, !kAll>{}, slow);
-        if constexpr (kAll)
-          order(PvProducts{}, integral_constant<int, 2>{}, integral_constant<int, 4>{}, integral_constant<int, 1>{});
-      }
-      if (!kAll && slow) {
-        // one key at a time, into the rows that see it
-#pragma unroll 1
-        for (int only = 0; only < KT; ++only) {
-          const int half_ = fresh(half);
-          float p = 0.f;   // in the half of the wave that holds the key
+        __builtin_amdgcn_sched_barrier(0);
+
+        // ---- softmax
+        if constexpr (!kAll) {
+          const int first = key0 + 4 * fresh(grp);
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) p = 32 * kb + (i & 3) + 8 * (i >> 2) == only - 4 * half_ ? s[kb][i] : p;
-          p = to_f32(from_f32<T>(half_sum(p)));
-          const bool take = key0 + only < lim && !hidden(key0 + only);
+            for (int i = 0; i < kAcc; ++i) {
+              const int key = first + RW * kb + index(i, 0);
+              bool see = key < lim;
+              if (bad_pages) see = see && !hidden(key);
+              s[kb][i] = see ? s[kb][i] : -INFINITY;
+            }
+        }
+        float t = s[0][0], u = s[0][1];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < kAcc; i += 4) {
+            t = fmaxf(fmaxf(t, s[kb][i]), s[kb][i + 1]);
+            u = fmaxf(fmaxf(u, s[kb][i + 2]), s[kb][i + 3]);
+          }
+        t = col_max<RW>(fmaxf(t, u)) * a.scale_log2;
+        const bool bump = t > m + kLazy;
+        if (__any(bump)) {
+          const float mn = bump ? t : m;
+          const float alpha = bump ? exp2_hw(m - mn) : 1.f;
+          m = mn;
+          l *= alpha;
 #pragma unroll
           for (int d = 0; d < NB; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int at = min(32 * d + (i & 3) + 8 * (i >> 2) + 4 * half_, D - 1) * (int)sizeof(T);
-              const T v = *reinterpret_cast<const T*>(vs + only * kRowB + (((at >> 4) ^ swz(only)) << 4) + (at & 15));
-              acc[d][i] = take ? __builtin_fmaf(p, to_f32(v), acc[d][i]) : acc[d][i];
+            for (int i = 0; i < kAcc; ++i) acc[d][i] *= alpha;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;   // (a row that has seen nothing yet: its terms are 0)
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < kAcc; ++i) {
+            s[kb][i] = exp2_hw(__builtin_fmaf(s[kb][i], a.scale_log2, -ref));
+            sum[i & 3] += s[kb][i];
+          }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if constexpr (WR == 1) {
+          if (more) vm_wait<kLoads>(); else vm_wait<0>();
+          if (edge) clear(tile, 0, true);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+
+        // ---- output
+        bool slow = false;
+        if (!kAll && ragged) {
+          // a value that is not finite in this tile?
+          uint32_t odd = 0;
+          for (int i = fresh(lane); i < KT * kPieces; i += 64) {
+            const u32x4 x = ld16(vs + 16 * i);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              if constexpr (kF32) {
+                odd |= (x[w] & 0x7f800000u) == 0x7f800000u;
+              } else {
+                constexpr uint32_t kExp = std::is_same<T, half_t>::value ? 0x7c00u : 0x7f80u;
+                odd |= (x[w] & kExp) == kExp;
+                odd |= ((x[w] >> 16) & kExp) == kExp;
+              }
             }
+          }
+          slow = __any(odd);
         }
-      }
-      if constexpr (WR == 1) {
-        if (more) {
-          lds_wait();
-          issue(tile + BN, 0, true);
+        // (with slow the product is taken of zeros, and the keys one at a time below)
+        const uint32_t mask = !kAll && slow ? 0u : ~0u;
+        if constexpr (kF32) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < kAcc; ++i) {
+              const int row = RW * kb + index(i, grp);
+#pragma unroll
+              for (int d = 0; d < NB; ++d) {
+                const int dim = min(RW * d + col, D - 1);   // (outputs past D are not used)
+                uint32_t v =
+                    *reinterpret_cast<const uint32_t*>(vs + row * kRowB + (((dim >> 2) ^ swz(row)) << 4) + (dim & 3) * 4);
+                uint32_t p = __float_as_uint(s[kb][i]);
+                if constexpr (!kAll) {
+                  v &= mask;
+                  p &= mask;
+                }
+                acc[d] = M_::one(__uint_as_float(v), __uint_as_float(p), acc[d]);
+              }
+            }
+        } else {
+          typedef __attribute__((address_space(3))) shortx4 lds4;
+          constexpr int kFar = RW == 32 ? 8 : 16;   // the second four of a lane's keys
+#pragma unroll
+          for (int h = 0; h < KT / kPk; ++h) {
+            // probabilities as they stand: element j is key kPk h + 4 grp + (j & 3) + kFar (j / 4)
+            frag p;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              p[j] = from_f32<T>(RW == 32 ? s[h / 2][(8 * (h & 1) + j) % kAcc] : s[(2 * h + j / 4) % KB][j % 4]);
+            if constexpr (!kAll) p = __builtin_bit_cast(frag, __builtin_bit_cast(u32x4, p) & mask);
+            const int row = kPk * h + 4 * grp + ((lane & 15) >> 2);
+#pragma unroll
+            for (int d = 0; d < NB; ++d) {
+              // dimensions past D (16) read the row's first ones; their output is not used
+              const int dim = (D % RW == 0 ? RW * d + (RW == 32 ? 16 * ((lane >> 4) & 1) : 0) : 0) + 4 * (lane & 3);
+              union {
+                shortx4 h[2];
+                u32x4 w;
+              } v;
+              v.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (lds4*)(vs + row * kRowB + (((dim >> 3) ^ swz(row)) << 4) + (dim & 4) * 2));
+              v.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (lds4*)(vs + (row + kFar) * kRowB + (((dim >> 3) ^ swz(row + kFar)) << 4) + (dim & 4) * 2));
+              if constexpr (!kAll) v.w &= mask;
+              acc[d] = M_::mma(__builtin_bit_cast(frag, v.w), p, acc[d]);
+            }
+          }
+          if constexpr (kAll)
+            order(integral_constant<int, KT / kPk * NB>{}, integral_constant<int, 2>{}, integral_constant<int, 4>{},
+                  integral_constant<int, 1>{});
         }
-      }
-    };
-    if (tile < send) {
+        if (!kAll && slow) {
+          // one key at a time, into the rows that see it
+#pragma unroll 1
+          for (int only = 0; only < KT; ++only) {
+            const int grp_ = fresh(grp);
+            float p = 0.f;   // in the lane of the column that holds the key
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+              for (int i = 0; i < kAcc; ++i) p = RW * kb + index(i, 0) == only - 4 * grp_ ? s[kb][i] : p;
+            p = to_f32(from_f32<T>(col_sum<RW>(p)));
+            const bool take = key0 + only < lim && !hidden(key0 + only);
+#pragma unroll
+            for (int d = 0; d < NB; ++d)
+#pragma unroll
+              for (int i = 0; i < kAcc; ++i) {
+                const int at = min(RW * d + index(i, 0) + 4 * grp_, D - 1) * (int)sizeof(T);
+                const T v = *reinterpret_cast<const T*>(vs + only * kRowB + (((at >> 4) ^ swz(only)) << 4) + (at & 15));
+                acc[d][i] = take ? __builtin_fmaf(p, to_f32(v), acc[d][i]) : acc[d][i];
+              }
+          }
+        }
+        if constexpr (WR == 1) {
+          if (more) {
+            lds_wait();
+            issue(tile + BN, 0, true);
+          }
+        }
+      };
       int n = 0;
       issue(tile, 0, false);
       issue(tile, 0, true);
+      // (the query rows are waited for here, once: in the loop the compiler's wait
+      // would be for every load in flight)
+#pragma unroll
+      for (int t = 0; t < NQ; ++t) asm volatile("" : "+v"(qw[t]));
 #pragma unroll 1
       for (; tile + BN <= whole; tile += BN, ++n) do_tile(n, std::true_type{});
 #pragma unroll 1
       for (; tile < send; tile += BN, ++n) do_tile(n, std::false_type{});
     }
-  }
-
   };
+
+  if ((a.q_xor | ~a.q_and) != 0) {   // a scaling below or of zero
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) qw[t] = (qw[t] & a.q_and) ^ a.q_xor;
+  }
   if constexpr (kMode == kPromptItem) {
     int lim = it.pend, all = it.pend, kend = it.pend;
     if (a.prefix_lens) {
@@ -606,7 +645,7 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, const Item& it,
       // keys every row of the workgroup sees, and keys some row sees
       int lo = lim, hi = live ? lim : 0;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
+      for (int o = RW / 2; o > 0; o >>= 1) {
         lo = min(lo, __shfl_xor(lo, o, 64));
         hi = max(hi, __shfl_xor(hi, o, 64));
       }
@@ -636,38 +675,38 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, const Item& it,
 
   // ---- the waves of the same rows join: through LDS, each row's sums weighted
   // by its waves' maxima
-  l = half_sum(l);
+  l = col_sum<RW>(l);
   constexpr int kOs = D + 4;
   float* so = reinterpret_cast<float*>(smem);
   __syncthreads();   // no tile is read any more
   if (live) {
-    if (half == 0) {
-      s_ml[(wave * 32 + col) * 2] = m;
-      s_ml[(wave * 32 + col) * 2 + 1] = l;
+    if (grp == 0) {
+      s_ml[(wave * RW + col) * 2] = m;
+      s_ml[(wave * RW + col) * 2 + 1] = l;
     }
 #pragma unroll
     for (int d = 0; d < NB; ++d)
 #pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        const int dim = 32 * d + 8 * (i >> 2) + 4 * half;
-        if (D % 32 == 0 || dim < D)
-          *reinterpret_cast<floatx4*>(so + (wave * 32 + col) * kOs + dim) =
+      for (int i = 0; i < kAcc; i += 4) {
+        const int dim = RW * d + index(i, grp);
+        if (D % RW == 0 || dim < D)
+          *reinterpret_cast<floatx4*>(so + (wave * RW + col) * kOs + dim) =
               floatx4{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
       }
   }
   __syncthreads();
   const int64_t rows_all = (int64_t)a.N * a.Hq;
   constexpr int kVec = D / 4;                    // 16-byte pieces of a row
-  const int first = it.row0 + 32 * wr, join = min(32, it.rows - first);   // the waves' live rows
+  const int first = it.row0 + RW * wr, join = min(RW, it.rows - first);   // the waves' live rows
   for (int i = wk * 64 + lane; i < join * kVec; i += 64 * WK) {
     const int c = i / kVec, dim = (i % kVec) * 4;
     float M = -INFINITY, L = 0.f;
     floatx4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < WK; ++k) M = fmaxf(M, s_ml[((k * WR + wr) * 32 + c) * 2]);
+    for (int k = 0; k < WK; ++k) M = fmaxf(M, s_ml[((k * WR + wr) * RW + c) * 2]);
 #pragma unroll
     for (int k = 0; k < WK; ++k) {
-      const int w = (k * WR + wr) * 32 + c;
+      const int w = (k * WR + wr) * RW + c;
       const float mk = s_ml[w * 2], scale = mk == -INFINITY ? 1.f : exp2_hw(mk - M);   // (no max: 0, or NaN)
       L += s_ml[w * 2 + 1] * scale;
       x += *reinterpret_cast<const floatx4*>(so + w * kOs + dim) * scale;
@@ -686,6 +725,21 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, const Item& it,
   }
 }
 
+// The items of one kind, by the rows of their tiles.
+template <typename T, int D, int kMode>
+__device__ __forceinline__ void prefix_items(int rows, const PrefixArgs& a, const Item& it, char* smem, int32_t* s_pid,
+                                             float* s_ml) {
+  switch (rows) {
+    case 16: prefix_item<T, D, 16, 1, kMode>(a, it, smem, s_pid, s_ml); break;
+    case 32: prefix_item<T, D, 32, 1, kMode>(a, it, smem, s_pid, s_ml); break;
+    case 64: prefix_item<T, D, 32, 2, kMode>(a, it, smem, s_pid, s_ml); break;
+    case 128: prefix_item<T, D, 32, 4, kMode>(a, it, smem, s_pid, s_ml); break;
+    default:
+      if constexpr (PrefixShape<T, D>::NW >= 8) prefix_item<T, D, 32, 8, kMode>(a, it, smem, s_pid, s_ml);
+      break;
+  }
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__((PrefixShape<T, D>::NW * 64)) __attribute__((amdgpu_waves_per_eu(1, 2))) void
 prefix_attn_kernel(PrefixArgs a) {
@@ -701,20 +755,13 @@ prefix_attn_kernel(PrefixArgs a) {
     const int per = a.Hk * a.p_splits, pair = x % per;
     it.hk = pair % a.Hk;
     const int split = pair / a.Hk;
-    it.row0 = x / per * 32 * a.p_wr;
+    it.row0 = x / per * a.p_rows;
     it.rows = tokens * a.G;
     it.pbeg = split * a.p_chunk;
     it.pend = min(a.S, it.pbeg + a.p_chunk);
     it.slot = a.o_splits + split;
     if (it.row0 >= it.rows) return;
-    switch (a.p_wr) {
-      case 1: prefix_item<T, D, 1, kPromptItem>(a, it, smem, s_pid, s_ml); break;
-      case 2: prefix_item<T, D, 2, kPromptItem>(a, it, smem, s_pid, s_ml); break;
-      case 4: prefix_item<T, D, 4, kPromptItem>(a, it, smem, s_pid, s_ml); break;
-      default:
-        if constexpr (NW >= 8) prefix_item<T, D, 8, kPromptItem>(a, it, smem, s_pid, s_ml);
-        break;
-    }
+    prefix_items<T, D, kPromptItem>(a.p_rows, a, it, smem, s_pid, s_ml);
   } else {
     x -= a.p_items;
     it.hk = x % a.Hk;
@@ -730,49 +777,39 @@ prefix_attn_kernel(PrefixArgs a) {
     }
     const int n = c1 - c0, len = min(max(a.lens[b], 0), a.T << a.lp);
     it.tok0 = c0;
-    it.row0 = tile * 32 * a.o_wr;
+    it.row0 = tile * a.o_rows;
     it.rows = min(n, a.max_new) * a.G;
     if (it.row0 >= it.rows) return;
     const int chunk = own_chunk(len, a.o_splits);
     it.lim0 = len - n + 1;
     it.obeg = min((int64_t)split * chunk, (int64_t)len);
-    const int last = min(it.row0 + 32 * a.o_wr, it.rows) - 1;   // the tile's row that sees most
+    const int last = min(it.row0 + a.o_rows, it.rows) - 1;   // the tile's row that sees most
     it.oend = min(min(it.obeg + chunk, len), max(0, it.lim0 + last / a.G));
     it.table = a.tables + b * a.t_sb;
     it.slot = split;
     if (a.both) {
       it.oend = min(len, max(0, it.lim0 + last / a.G));
       it.pend = a.prefix_lens ? min(max(a.prefix_lens[b], 0), a.S) : a.S;
-      switch (a.o_wr) {
-        case 1: prefix_item<T, D, 1, kBothItem>(a, it, smem, s_pid, s_ml); break;
-        case 2: prefix_item<T, D, 2, kBothItem>(a, it, smem, s_pid, s_ml); break;
-        case 4: prefix_item<T, D, 4, kBothItem>(a, it, smem, s_pid, s_ml); break;
-        default:
-          if constexpr (NW >= 8) prefix_item<T, D, 8, kBothItem>(a, it, smem, s_pid, s_ml);
-          break;
-      }
+      prefix_items<T, D, kBothItem>(a.o_rows, a, it, smem, s_pid, s_ml);
       return;
     }
     if (it.obeg >= it.oend) return;
-    switch (a.o_wr) {
-      case 1: prefix_item<T, D, 1, kOwnItem>(a, it, smem, s_pid, s_ml); break;
-      case 2: prefix_item<T, D, 2, kOwnItem>(a, it, smem, s_pid, s_ml); break;
-      case 4: prefix_item<T, D, 4, kOwnItem>(a, it, smem, s_pid, s_ml); break;
-      default:
-        if constexpr (NW >= 8) prefix_item<T, D, 8, kOwnItem>(a, it, smem, s_pid, s_ml);
-        break;
-    }
+    prefix_items<T, D, kOwnItem>(a.o_rows, a, it, smem, s_pid, s_ml);
   }
 }
 
 // Joins the partials of every query row: grid m_tiles tiles of rows of each
-// request, D / 4 threads a row.  A partial exists where the row sees keys of
-// its range, and where it does not the row has nothing there.  The threads of a
-// row take a partial's (max, sum) each, so that all of them are one load deep;
-// then the outputs' loads, four dimensions a thread, go out eight at a time.
-template <typename T, int D>
+// request; kSub groups of D / 4 threads a row take every kSub-th partial.  A
+// partial exists where the row sees keys of its range, and where it does not the
+// row has nothing there.  The threads of a group take a partial's (max, sum)
+// each, so that all of them are one load deep; then the outputs' loads, four
+// dimensions a thread, go out eight at a time.  Several groups a row pay where
+// few rows have many partials (32 rows with 17 of them: the call 15.5 -> 13.0 us).
+template <typename T, int D, int kSub>
 __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
-  constexpr int kVec = D / 4, kRows = 256 / kVec;
+  constexpr int kVec = D / 4, kRows = 256 / kVec / kSub;
+  static_assert(kRows >= 1, "a row's groups fit a workgroup");
+  __shared__ floatx4 s_x[kSub > 1 ? 256 : 1];
   const int b = blockIdx.x / a.m_tiles, tile = blockIdx.x % a.m_tiles;
   int c0 = b, c1 = b + 1;
   if (a.cu) {
@@ -781,15 +818,15 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
     c1 = min(max(a.cu[b + 1], c0), tokens);
   }
   const int n = c1 - c0, len = min(max(a.lens[b], 0), a.T << a.lp);
-  const int j = threadIdx.x % kVec, dim = 4 * j;
-  const int i = tile * kRows + threadIdx.x / kVec;
+  const int j = threadIdx.x % kVec, dim = 4 * j, sub = threadIdx.x / kVec % kSub;
+  const int i = tile * kRows + threadIdx.x / kVec / kSub;
   const int t = i / a.Hq, h = i - t * a.Hq;
-  if (t >= min(n, a.max_new)) return;   // (a row's threads together)
+  const bool live = t < min(n, a.max_new);   // (a row's threads together)
   const int S = a.prefix_lens ? min(max(a.prefix_lens[b], 0), a.S) : a.S;
   const int own = max(0, len - n + 1 + t), chunk = own_chunk(len, a.o_splits);
   const int n_own = (own + chunk - 1) / chunk, n_pre = a.p_splits ? (S + a.p_chunk - 1) / a.p_chunk : 0;
   const int64_t rows_all = (int64_t)a.N * a.Hq, ridx = (int64_t)(c0 + t) * a.Hq + h;
-  const int count = n_own + n_pre;
+  const int count = live ? n_own + n_pre : 0;
   // partial s of the row: the own ones first, then the prompt's
   auto at = [&](int s) { return (s < n_own ? s : a.o_splits + s - n_own) * rows_all + ridx; };
   typedef float floatx2 __attribute__((ext_vector_type(2)));
@@ -805,27 +842,36 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
     const float w = ml[0] == -INFINITY ? 1.f : exp2_hw(ml[0] - M);   // (sums without a max are 0, or NaN)
     if (s0 + j < count) L += ml[1] * w;
     const int todo = min(kVec, count - s0);
-    for (int k0 = 0; k0 < todo; k0 += 8) {
+    for (int k0 = sub; k0 < todo; k0 += 8 * kSub) {
       floatx4 o[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        o[k] = *reinterpret_cast<const floatx4*>(a.part_o + at(s0 + min(k0 + k, todo - 1)) * D + dim);
+        o[k] = *reinterpret_cast<const floatx4*>(a.part_o + at(s0 + min(k0 + k * kSub, todo - 1)) * D + dim);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float wk = __shfl(w, (k0 + k) % kVec, kVec);
-        if (k0 + k < todo) x += o[k] * wk;
+        const float wk = __shfl(w, (k0 + k * kSub) % kVec, kVec);
+        if (k0 + k * kSub < todo) x += o[k] * wk;
       }
     }
   }
 #pragma unroll
   for (int o = kVec / 2; o > 0; o >>= 1) L += __shfl_xor(L, o, 64);
-  finish_row<T>(a, c0 + t, h, dim, x, M, L);
+  if constexpr (kSub > 1) {
+    s_x[threadIdx.x] = x;
+    __syncthreads();
+    if (sub != 0) return;
+#pragma unroll
+    for (int k = 1; k < kSub; ++k) x += s_x[threadIdx.x + k * kVec];
+  }
+  if (live) finish_row<T>(a, c0 + t, h, dim, x, M, L);
 }
 
 template <typename T, int D>
 void launch_prefix_d(const PrefixArgs& a, int64_t items, hipStream_t s) {
   prefix_attn_kernel<T, D><<<(unsigned)items, PrefixShape<T, D>::NW * 64, 0, s>>>(a);
-  if (!a.both) prefix_merge_kernel<T, D><<<(unsigned)(a.B * a.m_tiles), 256, 0, s>>>(a);
+  if (a.both) return;
+  if (a.m_sub > 1) prefix_merge_kernel<T, D, kMergeSub><<<(unsigned)(a.B * a.m_tiles), 256, 0, s>>>(a);
+  else prefix_merge_kernel<T, D, 1><<<(unsigned)(a.B * a.m_tiles), 256, 0, s>>>(a);
 }
 
 template <typename T>
