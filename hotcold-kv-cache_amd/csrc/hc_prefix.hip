@@ -30,9 +30,9 @@ int tile_rows(int64_t rows, int waves) {
 // Times of a workgroup, in ns, as measured at head dimension 128 and 2-byte
 // types: kWgNs of its own (arguments, first loads, the waves' join), and a key's; kSweepNs of a
 // second run of keys, kJoinNs of the partials' join.
-// One CU streams about 40 GB/s, all together kHbm; products of 32 WR rows take
+// One CU streams about 40 GB/s, all together kHbm (paged and prompt rows at once); products of 32 WR rows take
 // the rest (30 ns a key of 256 rows).
-constexpr double kWgNs = 6500, kSweepNs = 3500, kJoinNs = 4500, kCuGBs = 40, kHbmGBs = 5000;
+constexpr double kWgNs = 6500, kSweepNs = 3500, kJoinNs = 4500, kCuGBs = 40, kHbmGBs = 4400;
 
 PrefixPlan plan_prefix(const hc_prefix_attn_args* x) {
   PrefixPlan p{};
@@ -58,19 +58,28 @@ PrefixPlan plan_prefix(const hc_prefix_attn_args* x) {
     // (a tile's keys, as in the kernel)
     const int wk = waves * 32 / std::max(32, p.p_rows);
     const int64_t bn = wk * (wk <= waves / 4 ? 64 : 32), units_p = p.p_tiles * x->Hk;
-    // Prompt items go first, and the own ones on the CUs they leave.  With s
-    // splits they take t; by then each CU left has done t / own_ns own items,
-    // and what remains of them runs on all CUs (or at the memory's rate).
+    // Prompt items go first, and the own ones on the CUs they leave; what these
+    // have not done by the prompt's end runs on all CUs.  Where both together
+    // ask for more than the memory gives, a CU that asks for less than its even
+    // part has all it asks for, and the others share the rest.
+    const double rate_p = key_bytes / key_ns(p.p_rows), rate_o = key_bytes / key_ns(p.o_rows);
     double best = 0;
     for (int64_t s = 1; s <= 512; s += 1 + s / 12) {
       const int64_t chunk = cdiv(cdiv(x->prefix_rows, s), bn) * bn, splits = cdiv(x->prefix_rows, chunk);
-      const double n = (double)(units_p * splits), rounds = std::ceil(n / kCus);
-      const double left = std::max(0.0, kCus - n);
-      double t = rounds * (kWgNs + (double)chunk * key_ns(p.p_rows));
-      const double done = std::min(own_n, left * std::floor(t / own_ns));
-      t = std::max(t, (n * (double)chunk + done * own_keys) * key_bytes / kHbmGBs);
-      const double rest = own_n - done;
-      if (rest > 0) t += std::max(std::ceil(rest / kCus) * own_ns, rest * own_keys * key_bytes / kHbmGBs);
+      const double n = (double)(units_p * splits), busy = std::min(n, (double)kCus), left = kCus - busy;
+      const double even = kHbmGBs / kCus, bytes_p = (double)chunk * key_bytes, bytes_o = own_keys * key_bytes;
+      double gets_p = rate_p, gets_o = rate_o;
+      if (busy * rate_p + left * rate_o > kHbmGBs) {
+        gets_p = rate_o <= even ? (kHbmGBs - left * rate_o) / busy : std::min(rate_p, even);
+        if (left > 0) gets_o = rate_p <= even ? (kHbmGBs - busy * rate_p) / left : std::min(rate_o, even);
+      }
+      const double beside = kWgNs + bytes_o / gets_o, all_o = left > 0 ? own_n * beside / left : 1e18;
+      double t = kWgNs + bytes_p / gets_p;
+      if (t > all_o) t = all_o + std::max(0.0, t - all_o) * gets_p / std::min(rate_p, kHbmGBs / busy);
+      t *= std::ceil(n / kCus);
+      const double rest = std::max(0.0, own_n - left * t / beside);
+      if (rest > 0)   // (the last to end may be a request of twice the mean length)
+        t += std::max(rest / kCus * own_ns, rest * bytes_o / kHbmGBs) + own_ns - kWgNs;
       t += (double)(splits * rows * x->Hk * x->D * 8) / kHbmGBs;   // partials, written and read
       if (p.p_splits == 0 || t < best) {
         best = t;
