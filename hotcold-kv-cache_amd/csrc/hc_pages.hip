@@ -60,9 +60,10 @@ __device__ __forceinline__ int64_t pages_of(int64_t rows, int lp) { return (rows
 // list; the token on a page's first row writes the table entry (each new page
 // has exactly one such token, and old entries are never written, so the
 // workgroups share nothing).
-//   kFill: write tables, slots, positions and cu; kCommit: write lens_out and
-//   count_out.  One workgroup does both; with several, a second launch of one
-//   workgroup commits, so lens_out may be lens and count_out free_count.
+//   kFill: write tables, slots, positions and cu; kCommit: the first workgroup
+//   writes lens_out and count_out.  Where several workgroups read the lengths
+//   and the count that this replaces (lens_out is lens, or count_out
+//   free_count), a second launch of one workgroup commits.
 // Bound by latency: two dependent loads and two scans (a step of 16 requests);
 // per token 16 bytes are written (a batch of prompts).
 template <bool kFill, bool kCommit>
@@ -74,6 +75,7 @@ __global__ __launch_bounds__(kPageThreads) void extend_pages_kernel(ExtendArgs a
   __shared__ uint32_t s_sums[kPageThreads / 64];
   constexpr uint32_t kNone = 0xffffffffu;
   const int tid = threadIdx.x;
+  const bool commit = kCommit && blockIdx.x == 0;
   const int count = min(max(*a.free_count, 0), a.F);
   const uint32_t N = (uint32_t)a.N;
   uint32_t tok0 = 0, page0 = 0, used = 0;
@@ -98,17 +100,17 @@ __global__ __launch_bounds__(kPageThreads) void extend_pages_kernel(ExtendArgs a
       s_before[b] = ok ? upto - need : kNone;
       s_len[b] = (int32_t)len;
       if (kFill && blockIdx.x == 0) a.cu[b + 1] = (int32_t)min(end, N);
-      if (kCommit) a.lens_out[b] = (int32_t)(ok ? len + more : len);
+      if (commit) a.lens_out[b] = (int32_t)(ok ? len + more : len);
     }
     // the largest sum that fits: sums never fall, so it is what was taken
-    if (kCommit) {
+    if (commit) {
       uint32_t u = fits ? upto : 0u;
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) u = max(u, (uint32_t)__shfl_xor((int)u, o, 64));
       used = max(used, u);
     }
   }
-  if (kCommit) {
+  if (commit) {
     __syncthreads();
     if ((tid & 63) == 0) s_sums[tid >> 6] = used;
     __syncthreads();
@@ -168,6 +170,7 @@ __global__ __launch_bounds__(kPageThreads) void release_pages_kernel(ReleaseArgs
   uint32_t* s_n = s_first + a.B;                   // [B]: pages given back
   __shared__ uint32_t s_sums[kPageThreads / 64];
   const int tid = threadIdx.x;
+  const bool commit = kCommit && blockIdx.x == 0;
   const int count = min(max(*a.free_count, 0), a.F);
   uint32_t page0 = 0;
   for (int b0 = 0; b0 < a.B; b0 += kPageThreads) {
@@ -185,10 +188,10 @@ __global__ __launch_bounds__(kPageThreads) void release_pages_kernel(ReleaseArgs
       s_before[b] = upto - n;
       s_first[b] = (uint32_t)first;
       s_n[b] = n;
-      if (kCommit) a.lens_out[b] = (int32_t)kept;
+      if (commit) a.lens_out[b] = (int32_t)kept;
     }
   }
-  if (kCommit && tid == 0) *a.count_out = (int)min((uint64_t)count + page0, (uint64_t)a.F);
+  if (commit && tid == 0) *a.count_out = (int)min((uint64_t)count + page0, (uint64_t)a.F);
   if (!kFill) return;
   __syncthreads();
   const int lane = tid & 63;
@@ -234,6 +237,9 @@ __global__ __launch_bounds__(256) void append_paged_kernel(AppendPagedArgs a) {
   }
 }
 
+// Whether [a, a + n) and [b, b + m) share a word.
+static bool meet(const int32_t* a, int64_t n, const int32_t* b, int64_t m) { return a < b + m && b < a + n; }
+
 // log2 of a page size, or -1
 int page_shift(int64_t P) {
   if (P < 1 || P > 65536 || (P & (P - 1)) != 0) return -1;
@@ -266,9 +272,14 @@ extern "C" int hc_extend_pages(int64_t B, const int32_t* lens, const int32_t* ne
                      (int)B, (int)table_width, (int)free_capacity, (int)N, lp};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const size_t lds = (3 * (size_t)B + 1) * 4;
-  const int64_t blocks = std::min<int64_t>(256, cdiv(N, (int64_t)kPageThreads));
-  if (blocks <= 8) {
-    extend_pages_kernel<true, true><<<1, kPageThreads, lds, s>>>(a);
+  // (a workgroup scans all requests before its first token: up to 8 tokens a
+  // thread one does it all)
+  int64_t blocks = std::min<int64_t>(256, cdiv(N, (int64_t)kPageThreads));
+  if (blocks <= 8) blocks = 1;
+  const bool in_place = meet(lens_out, B, lens, B) || meet(lens_out, B, new_lens, B) || meet(lens_out, B, free_count, 1) ||
+                        meet(count_out, 1, free_count, 1) || meet(count_out, 1, lens, B) || meet(count_out, 1, new_lens, B);
+  if (blocks == 1 || !in_place) {
+    extend_pages_kernel<true, true><<<(unsigned)blocks, kPageThreads, lds, s>>>(a);
     return check_launch("extend_pages");
   }
   extend_pages_kernel<true, false><<<(unsigned)blocks, kPageThreads, lds, s>>>(a);
@@ -297,11 +308,13 @@ extern "C" int hc_release_pages(int64_t B, const int32_t* lens, const int32_t* k
                       (int)B, (int)table_width, (int)free_capacity, lp};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const size_t lds = 3 * (size_t)B * 4;
-  if (B <= 32) {
-    release_pages_kernel<true, true><<<1, kPageThreads, lds, s>>>(a);
+  const int64_t blocks = B <= 32 ? 1 : std::min<int64_t>(256, cdiv(B, (int64_t)(kPageThreads / 64)));
+  const bool in_place = meet(lens_out, B, lens, B) || meet(lens_out, B, keep_lens, B) || meet(lens_out, B, free_count, 1) ||
+                        meet(count_out, 1, free_count, 1) || meet(count_out, 1, lens, B) || meet(count_out, 1, keep_lens, B);
+  if (blocks == 1 || !in_place) {
+    release_pages_kernel<true, true><<<(unsigned)blocks, kPageThreads, lds, s>>>(a);
     return check_launch("release_pages");
   }
-  const int64_t blocks = std::min<int64_t>(256, cdiv(B, (int64_t)(kPageThreads / 64)));
   release_pages_kernel<true, false><<<(unsigned)blocks, kPageThreads, lds, s>>>(a);
   if (const int rc = check_launch("release_pages")) return rc;
   release_pages_kernel<false, true><<<1, kPageThreads, lds, s>>>(a);

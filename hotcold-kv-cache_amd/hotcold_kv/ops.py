@@ -1187,7 +1187,9 @@ def inject_rerope_tab(k_pre, v_staged, cos_t, sin_t, k_dst, v_dst):
 # A batch of requests behind one shared prompt: pages and attention
 # ---------------------------------------------------------------------------
 def _stream_of(t):
-    return stream_handle(t.device) if t.is_cuda else 0
+    if not t.is_cuda:
+        return 0
+    return _raw_stream(t.get_device()) if _raw_stream is not None else stream_handle(t.device)
 
 
 def extend_pages(lens, new_lens, tables, free_pages, free_count, page_size, num_tokens, lens_out=None,
