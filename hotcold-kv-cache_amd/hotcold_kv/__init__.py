@@ -6,6 +6,7 @@ from .datatypes import RetrievedKV, EvictedKV
 from .kernels import triton_evict_attention_forward, decode_attention_forward
 from .controller import KVController
 from .cache import HotColdLayer, build_hotcold_cache
+from .paged import SharedPromptBatch
 from .patch import (
     set_active_kvctrl,
     set_active_rotary_emb,
@@ -22,6 +23,7 @@ __all__ = [
     "KVController",
     "HotColdLayer",
     "build_hotcold_cache",
+    "SharedPromptBatch",
     "set_active_kvctrl",
     "set_active_rotary_emb",
     "install_monkeypatch",

@@ -667,3 +667,129 @@ def test_a_captured_step_replays_over_new_lengths(tokens):
         for s in sides:
             for name in ("lens", "count", "tables", "out", "k_pages", "v_pages"):
                 assert torch.equal(s[name], eager[name]), (it, name)
+
+
+# ---------------------------------------------------------------------------
+# The operators as a serving loop uses them
+# ---------------------------------------------------------------------------
+def test_argument_struct_has_the_headers_fields():
+    import os
+    import re
+    path = os.path.join(os.path.dirname(__file__), "..", "include", "hotcold_hip.h")
+    with open(path) as f:
+        body = re.search(r"typedef struct hc_prefix_attn_args \{(.*?)\}", f.read(), re.S).group(1)
+    want = []
+    for decl in filter(None, (d.strip() for d in re.sub(r"/\*.*?\*/", "", body, flags=re.S).split(";"))):
+        kind = "p" if "*" in decl else "d" if decl.startswith("double") else "i"
+        names = re.sub(r"^(const )?(void|float|int32_t|int64_t|double)\s*\*?\s*", "", decl)
+        want += [(n.strip(), kind) for n in names.split(",")]
+    kinds = {N._vp: "p", N._dbl: "d", N._i64: "i"}
+    assert [(n, kinds[t]) for n, t in N.PrefixAttnArgs._fields_] == want
+
+
+def test_batch_refuses():
+    from hotcold_kv import SharedPromptBatch
+    from hotcold_kv.hot_buffer import HotBuffer
+    with pytest.raises(ValueError, match="at least 1"):
+        SharedPromptBatch(1, 0, 2, 64, torch.float16, "cpu", 8, 16, 64)
+    b = SharedPromptBatch(1, 2, 2, 64, torch.float16, "cpu", 8, 16, 64)
+    with pytest.raises(ValueError, match="batch 2"):
+        b.set_prompt(0, HotBuffer(2, 2, 64, torch.float16, "cpu", 4))
+    with pytest.raises(RuntimeError, match="before extend"):
+        b.attend(0, None, None, None, 1.0)
+    with pytest.raises(RuntimeError, match="device"):
+        b.extend(torch.ones(2, dtype=torch.int32), 2, 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,requests,Hq,Hk,D,P", [("f16", 5, 8, 2, 128, 16), ("bf16", 40, 6, 3, 64, 4), ("f32", 3, 4, 4, 16, 32)])
+def test_a_batch_behind_a_compacted_prompt(dtype, requests, Hq, Hk, D, P):
+    """Prompts, decode steps, rejected tokens, requests that end and others that take their rows, over two layers
+    whose prompts were compacted to different rows: every token against the 64-bit attention over a dense copy of
+    what its request holds."""
+    from hotcold_kv import SharedPromptBatch
+    from hotcold_kv.hot_buffer import HotBuffer
+    g = torch.Generator().manual_seed(11)
+    dt, layers, S, longest, most = DTYPES[dtype], 2, 200, 60, 20
+    pages = requests * -(-longest // P)
+    batch = SharedPromptBatch(layers, requests, Hk, D, dt, "cuda", pages, P, longest)
+    prompts = []
+    for layer in range(layers):
+        buf = HotBuffer(1, Hk, D, dt, "cuda", S)
+        k, v = (torch.randn((1, Hk, S, D), generator=g).to(dt) for _ in range(2))
+        buf.append(k.cuda(), v.cuda())
+        keep = torch.stack([torch.randperm(S, generator=g)[:90 + 40 * layer].sort().values for _ in range(Hk)])[None]
+        buf.compact(keep.cuda())
+        at = keep[..., None].expand(-1, -1, -1, D)
+        prompts.append((k.gather(2, at), v.gather(2, at)))
+        batch.set_prompt(layer, buf)
+    held = [0] * requests
+    dense = [[torch.zeros((requests, Hk, longest, D), dtype=dt) for _ in range(2)] for _ in range(layers)]
+    own = torch.arange(requests, dtype=torch.int32)[:, None]            # the dense copy is a pool of one page a request
+    for it in range(9):
+        new = [int(x) for x in torch.randint(1, most + 1, (requests,), generator=g)] if it % 4 == 0 else [1] * requests
+        new = [min(n, longest - h) for n, h in zip(new, held)]
+        if it == 5:
+            new[1] = 0                                                  # idle in this step
+        n = sum(new) + it % 3
+        pos = batch.extend(torch.tensor(new, dtype=torch.int32).cuda(), n, max(new))
+        held = [h + x for h, x in zip(held, new)]
+        assert batch.lens.tolist() == held
+        rows = [(b, held[b] - new[b] + i) for b in range(requests) for i in range(new[b])]
+        assert pos.tolist() == [r for _, r in rows] + [-1] * (n - len(rows))
+        cu = torch.tensor([0] + new).cumsum(0).int()
+        for layer in range(layers):
+            q = torch.randn((n, Hq, D), generator=g).to(dt)
+            k, v = (torch.randn((n, Hk, D), generator=g).to(dt) for _ in range(2))
+            for i, (b, r) in enumerate(rows):
+                dense[layer][0][b, :, r], dense[layer][1][b, :, r] = k[i], v[i]
+            out = torch.full((n, Hq, D), 7.0, dtype=dt, device="cuda")
+            batch.attend(layer, q.cuda(), k.cuda(), v.cuda(), D ** -0.5, out=out)
+            want = ref_attention(q, *prompts[layer], *dense[layer], own, torch.tensor(held), D ** -0.5, cu)
+            check_attention(out, want, dt)
+            assert bool((out[len(rows):] == 7).all())
+        if it % 2 == 1:                                                 # reject up to two tokens, end every fifth request
+            keep = [0 if (b + it) % 5 == 0 else max(h - b % 3, 0) for b, h in enumerate(held)]
+            batch.release(torch.tensor(keep, dtype=torch.int32).cuda())
+            held = keep
+            with pytest.raises(RuntimeError, match="before extend"):
+                batch.attend(0, q, k, v, 1.0)
+    batch.release(torch.zeros(requests, dtype=torch.int32).cuda())
+    assert batch.lens.tolist() == [0] * requests and batch.free_count.tolist() == [pages]
+    assert sorted(batch.free_pages.tolist()) == list(range(pages))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [3, 2500])
+@pytest.mark.parametrize("overlap", ["none", "lens", "count", "crossed"])
+def test_outputs_may_be_any_of_the_inputs(tokens, overlap):
+    """Lengths and count written over any input they replace, with one workgroup and with several."""
+    B, P, F = 40, 16, 400
+    lens, new = [3 * b % 50 for b in range(B)], [1 + (tokens // B if b % 2 else 0) for b in range(B)]
+    keep = [max(0, n - b % 30) for b, n in enumerate(lens)]
+    g = torch.Generator().manual_seed(tokens)
+    T = -(-(max(lens) + max(new)) // P)
+    tables, _, _ = _tables(g, lens, T, P, 0)
+    free = list(range(1000, 1000 + F))
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for op in ("extend", "release"):
+        count = 300
+        dl, dn, dk, dt, df, dc = (torch.tensor(x, **i32) for x in (lens, new, keep, tables, free, [count]))
+        lo, co = torch.zeros(B, **i32), torch.zeros(1, **i32)
+        more = dn if op == "extend" else dk
+        if overlap == "lens":
+            lo = dl
+        elif overlap == "count":
+            co = dc
+        elif overlap == "crossed":
+            lo, co = more, dc
+        if op == "extend":
+            n = sum(new)
+            want = ref_extend(lens, new, tables, free, count, P, n)
+            got = ops.extend_pages(dl, dn, dt, df, dc, P, n, lens_out=lo, count_out=co)
+            assert got[3].tolist() == want[3] and got[4].tolist() == want[4] and dt.tolist() == want[5]
+        else:
+            want = ref_release(lens, keep, tables, free, count, P)
+            ops.release_pages(dl, dk, dt, df, dc, P, lens_out=lo, count_out=co)
+            assert df.tolist() == want[2]
+        assert lo.tolist() == want[0] and co.tolist() == [want[1]]
