@@ -103,7 +103,7 @@ PrefixPlan plan_prefix(const hc_prefix_attn_args* x) {
     p.o_splits = 1;
   }
   const int64_t vec = x->D / 4;   // threads of a row's group
-  p.m_sub = x->D == 128 && x->B * cdiv(most * x->Hq * vec, (int64_t)256) < 2 * kCus && p.p_splits + p.o_splits >= 8 ? kMergeSub : 1;
+  p.m_sub = x->B * cdiv(most * x->Hq * vec, (int64_t)256) < 2 * kCus && p.p_splits + p.o_splits >= 8 ? kMergeSub : 1;
   p.m_tiles = (int)cdiv(most * x->Hq * vec * p.m_sub, (int64_t)256);
   p.items = (int64_t)p.p_tiles * x->Hk * p.p_splits + units * p.o_splits;
   p.slots = p.p_splits + p.o_splits;
