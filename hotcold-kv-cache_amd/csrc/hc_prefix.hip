@@ -28,10 +28,10 @@ int tile_rows(int64_t rows, int waves) {
 }
 
 // Times of a workgroup, in ns, as measured at head dimension 128 and 2-byte
-// types: kWgNs of its own (arguments, first loads, the waves' join), and a key's; kSweepNs of a
-// second run of keys, kJoinNs of the partials' join.
-// One CU streams about 40 GB/s, all together kHbm (paged and prompt rows at once); products of 32 WR rows take
-// the rest (30 ns a key of 256 rows).
+// types: kWgNs of its own (arguments, first loads, the waves' join), and a
+// key's; kSweepNs of a second run of keys, kJoinNs of the partials' join.  One
+// CU streams about 40 GB/s, all together kHbmGBs (paged and prompt rows at
+// once); products of 32 WR rows take the rest (30 ns a key of 256 rows).
 constexpr double kWgNs = 6500, kSweepNs = 3500, kJoinNs = 4500, kCuGBs = 40, kHbmGBs = 4400;
 
 PrefixPlan plan_prefix(const hc_prefix_attn_args* x) {
@@ -106,7 +106,7 @@ PrefixPlan plan_prefix(const hc_prefix_attn_args* x) {
   p.m_sub = x->B * cdiv(most * x->Hq * vec, (int64_t)256) < 2 * kCus && p.p_splits + p.o_splits >= 8 ? kMergeSub : 1;
   p.m_tiles = (int)cdiv(most * x->Hq * vec * p.m_sub, (int64_t)256);
   p.items = (int64_t)p.p_tiles * x->Hk * p.p_splits + units * p.o_splits;
-  p.slots = p.p_splits + p.o_splits;
+  p.slots = p.both ? 0 : p.p_splits + p.o_splits;   // (rows written complete need no partials)
   return p;
 }
 
@@ -174,8 +174,9 @@ extern "C" int hc_prefix_attn(const hc_prefix_attn_args* x, void* stream) {
                      (long long)(x->workspace ? x->workspace_bytes : 0), (long long)need);
   HC_REQUIRE((uintptr_t)x->workspace % 16 == 0, "prefix_attention: the workspace must be 16-byte aligned");
   const PrefixPlan p = plan_prefix(x);
-  HC_REQUIRE(p.items <= INT32_MAX && x->B * p.m_tiles <= INT32_MAX, "prefix_attention: %lld workgroups",
-             (long long)p.items);
+  // (a grid's threads are counted in 32 bits)
+  HC_REQUIRE(p.items <= UINT32_MAX / 512 && x->B * p.m_tiles <= UINT32_MAX / 256, "prefix_attention: %lld workgroups",
+             (long long)std::max(p.items, x->B * p.m_tiles));
   const int dtype = (int)x->dtype;
   const int64_t es = dtype_size(dtype);
   PrefixArgs a{};

@@ -1258,8 +1258,8 @@ def prefix_attention(q, k_prefix, v_prefix, k_pages, v_pages, tables, lens, scal
     request.  The prompt's keys and values are read once for all requests.
 
     Returns out (N,Hq,D) in q's dtype, with return_lse also the fp32 natural
-    log-sum-exp (N,Hq).  A token that attends nothing gets zeros and -inf.  Rows
-    behind the last request are not written."""
+    log-sum-exp (N,Hq).  A token that attends nothing, or whose logits are all
+    -inf, gets zeros and -inf.  Rows behind the last request are not written."""
     o, lse, rc = N.tensor_bind().prefix_attention(q, k_prefix, v_prefix, k_pages, v_pages, tables, lens,
                                                   scaling, cu_new, max_new, prefix_lens, out, return_lse,
                                                   _stream_of(q))

@@ -57,7 +57,7 @@ class SharedPromptBatch:
         self.lens, self.free_count, cu, slots, pos = ops.extend_pages(
             self.lens, new_lens, self.tables, self.free_pages, self.free_count, self.page_size, num_tokens,
             lens_out=self.lens, count_out=self.free_count)
-        self._step = (cu, slots, int(max_new))
+        self._step = (cu, slots, max(1, int(max_new)))   # (a step of no tokens attends nothing)
         return pos
 
     def attend(self, layer, q, k, v, scaling, prefix_lens=None, out=None, return_lse=False):

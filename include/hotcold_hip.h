@@ -740,8 +740,9 @@ int hc_append_paged(int dtype, int64_t N, int64_t Hk, int64_t D, const int64_t* 
  * already hold them).  Token i of n attends the prompt's rows
  * 0 .. prefix_lens[b] (NULL: all prefix_rows) and its own rows
  * 0 .. lens[b] - n + i, its own row last.  A table entry outside the pool hides its
- * page's rows.  A token that attends nothing gets zeros (lse -inf).  Rows of
- * out (and lse) behind the last request are left as they were.
+ * page's rows.  A token that attends nothing, or whose logits are all -inf,
+ * gets zeros (lse -inf).  Rows of out (and lse) behind the last request are
+ * left as they were.
  *   k_prefix, v_prefix [Hk][prefix_rows][D] (NULL when prefix_rows == 0)
  *   out [N][Hq][D] in dtype; lse [N][Hq] fp32 (may be NULL): the natural
  *     logarithm of the softmax's sum of exponentials.
