@@ -94,11 +94,13 @@ PrefixPlan plan_prefix(const hc_prefix_attn_args* x) {
   // Or each own item takes the prompt as well: no partials, but the prompt once
   // for every request's tile.  (Requests' own prompts of up to 512 tokens behind
   // 64 rows: 94 us -> 61.  Of 1024 behind 8192, where the estimates are close:
-  // 802 us apart, 963 together.)
+  // 802 us apart, 963 together.)  With no prompt and one item a row nothing is joined
+  // (256 requests of up to 1024 rows: 145 -> 138 us; 8 prompts of up to
+  // 512 tokens: 116 -> 88).
   const double both = std::ceil(tiles * (double)x->Hk / kCus) *
                       (kWgNs + (x->prefix_rows > 0 ? kSweepNs : 0) +
                        ((double)x->prefix_rows + 0.5 * (double)longest) * key_ns(p.o_rows));
-  if ((p.both = both < 0.9 * two)) {
+  if ((p.both = both < 0.9 * two || (x->prefix_rows == 0 && p.o_splits == 1))) {
     p.p_tiles = p.p_splits = 0;
     p.o_splits = 1;
   }
