@@ -793,3 +793,46 @@ def test_outputs_may_be_any_of_the_inputs(tokens, overlap):
             ops.release_pages(dl, dk, dt, df, dc, P, lens_out=lo, count_out=co)
             assert df.tolist() == want[2]
         assert lo.tolist() == want[0] and co.tolist() == [want[1]]
+
+
+def test_library_refuses_grids_past_32_bits():
+    import ctypes
+    a = _attn_args(N=65536, B=65536, Hq=1024, Hk=1024, D=16, workspace=4096, workspace_bytes=1 << 60)
+    assert N.lib().hc_prefix_attn(ctypes.addressof(a), None) == N.HC_ERR_INVALID
+    assert b"workgroups" in N.lib().hc_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("requests,new,D,share", [(33, 1, 64, False), (70, 1, 128, True), (29, 3, 32, True), (9, 16, 128, False)])
+def test_query_rows_that_do_not_fill_a_tile(dtype, requests, new, D, share):
+    """Batches whose query rows leave waves of a tile, or of the last one, without any."""
+    g = torch.Generator().manual_seed(requests)
+    lens = [int(x) for x in torch.randint(new, 40, (requests,), generator=g)]
+    c = paged_case(dtype, lens, [new] * requests, prefix=1500, Hq=8, Hk=2, D=D, P=8, seed=requests)
+    if new == 1:
+        c["cu"] = None
+    limits = torch.randint(0, 1501, (requests,), generator=g).int() if share else None
+    d = to_dev(c)
+    got, lse = attend(d, prefix_lens=None if limits is None else limits.cuda(), return_lse=True)
+    check_attention(got, want_attention(c, limits), DTYPES[dtype], lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("prefix", [None, 0])
+@pytest.mark.parametrize("lens,new", [([1], [1]), ([300, 0, 7, 64] * 40, [1] * 160), ([500, 3, 129] * 24, [200, 3, 1] * 24)])
+def test_requests_without_a_prompt(dtype, prefix, lens, new):
+    c = paged_case(dtype, lens, new, prefix=prefix, Hq=4, Hk=2, D=64, P=16, seed=len(lens))
+    got, lse = attend(to_dev(c), return_lse=True)
+    check_attention(got, want_attention(c), DTYPES[dtype], lse)
+
+
+@pytest.mark.gpu
+def test_a_step_of_no_tokens():
+    from hotcold_kv import SharedPromptBatch
+    b = SharedPromptBatch(1, 3, 2, 64, torch.float16, "cuda", 4, 16, 32)
+    assert b.extend(torch.zeros(3, dtype=torch.int32, device="cuda"), 0, 0).shape == (0,)
+    z = torch.zeros((0, 2, 64), dtype=torch.float16, device="cuda")
+    assert b.attend(0, torch.zeros((0, 8, 64), dtype=torch.float16, device="cuda"), z, z, 1.0).shape == (0, 8, 64)
+    assert b.lens.tolist() == [0, 0, 0] and b.free_count.tolist() == [4]
